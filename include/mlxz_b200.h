@@ -63,7 +63,9 @@ enum mz_device_error {
   MZ_DEVERR_SLOT = 2,     /* slot outside [0, n_blocks * block_size)          */
   MZ_DEVERR_CONTEXT = 4,  /* context length < 0 or > table capacity           */
   MZ_DEVERR_TIMEOUT = 8,  /* a bounded wait on an mbarrier or flag gave up    */
-  MZ_DEVERR_ROWS = 16     /* a sequence's query rows outside [0, n_rows)      */
+  MZ_DEVERR_ROWS = 16,    /* a sequence's query rows outside [0, n_rows)      */
+  MZ_DEVERR_BLOCKS = 32,  /* more new blocks needed than were given           */
+  MZ_DEVERR_AXIS = 64     /* a frequency's position axis outside [0, n_axes)  */
 };
 
 /* ABI version of this header (bumped on any signature change). */
@@ -104,6 +106,74 @@ MZ_API int mz_kv_append_paged(void *k_pool, void *v_pool, const void *k_new, con
                        const int32_t *positions, int32_t n_seqs, int32_t n_kv_heads,
                        int32_t head_dim, int32_t block_size, int64_t n_blocks, int32_t dtype,
                        int32_t *dev_err, mz_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
+/* Step metadata on the GPU.                                                 */
+/* ------------------------------------------------------------------------ */
+
+/* Block tables, slot maps and positions of a step from the requests' lengths,
+ * in one launch.  Sequence b holds ctx_lens[b] tokens in held[b] blocks (NULL:
+ * ceil(ctx / block_size)) and gets q_lens[b] new ones:
+ *   need_b     = max(0, ceil((ctx_lens[b] + q_lens[b]) / block_size) - held[b]),
+ *   block_tables[b][held[b] + i] = the next of new_ids, sequence by sequence
+ *                (the order in which BlockManager.allocate hands blocks out),
+ *   q_start[b] = q_lens[0] + ... + q_lens[b - 1],
+ *   row q_start[b] + i: positions = ctx_lens[b] + i, slots = the pool slot of
+ *                that position (mz_kv_append's slot_mapping),
+ *   lengths[b] = ctx_lens[b] + q_lens[b],  held_out[b] = held[b] + need_b,
+ *   n_used[0]  = sum of need_b.
+ * Rows from sum(q_lens) to n_rows (a padded batch) get slot -1, which the
+ * appends skip, and position 0.  Replaces the host's walk over tables and
+ * tokens: PagedKVCache.append_kv, src/mlxz/paged_attention/paged_kv.py:72-83.
+ * Reported and skipped (no rows, the sequence's lengths and held stay): lengths
+ * that are negative, exceed the table, or exceed held blocks' tokens with
+ * ctx_lens (MZ_DEVERR_CONTEXT); rows past n_rows (MZ_DEVERR_ROWS).  Slots
+ * without a valid block are -1 and reported (MZ_DEVERR_BLOCK_ID; _BLOCKS when
+ * new_ids run out).  Outputs must not overlap inputs. */
+MZ_API int mz_paged_plan(int32_t *block_tables, int32_t max_blocks_per_seq,
+                         const int32_t *ctx_lens, const int32_t *q_lens, const int32_t *held,
+                         const int32_t *new_ids, int32_t n_new_ids, int32_t n_seqs,
+                         int32_t n_rows, int32_t block_size, int64_t n_blocks, int32_t *q_start,
+                         int32_t *positions, int64_t *slots, int32_t *lengths, int32_t *held_out,
+                         int32_t *n_used, int32_t *dev_err, mz_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
+/* Query / key norm, rotation and append.                                    */
+/* ------------------------------------------------------------------------ */
+
+/* RMS norm of every query and key head, rotation by position, and the write of
+ * K and V to their cache slots, in one pass over q, k and v:
+ *   y = x / sqrt(mean(x^2) + eps) * (w + weight_offset)   per head, if `norm`
+ *       (a NULL weight: no multiplication),
+ *   theta_i = positions[axis_i][token] * inv_freq[i],  0 <= i < rot_dim / 2,
+ *   pair i -> (a cos theta_i - b sin theta_i, b cos theta_i + a sin theta_i),
+ * with pair i = dims (i, i + rot_dim / 2), or (2 i, 2 i + 1) if `interleaved`;
+ * dims from rot_dim on keep y.  axis_i = freq_axes[i] (NULL: 0; several axes,
+ * e.g. time / height / width of image tokens, each a row of `positions`
+ * pos_axis_stride apart; an axis outside [0, n_axes): MZ_DEVERR_AXIS, axis 0).
+ * fp32 throughout (angles in fp64 before their reduction), rounded once.
+ * Element (token t, head h, dim d) of a tensor at t*tok_stride + h*head_stride
+ * + d.  q_out (may be q itself) gets the queries.  With pools, k's result and v
+ * go to slot_mapping[t] of k_pool / v_pool as in mz_kv_append (negative: K/V
+ * skipped; too large: MZ_DEVERR_SLOT), and k_out must be NULL; without, k's
+ * result goes to k_out (may be k) and v is not read.  Slots of one call must
+ * be distinct.  Takes the place of the q_norm / k_norm / rope calls of the
+ * model's attention layer and the cache.update_and_fetch after them
+ * (src/mlxz/engine/continuous.py:625-633 runs them inside the model).
+ * Supported: F16 / BF16 / F32; head_dim a multiple of 16 up to 256; rot_dim a
+ * multiple of 16 up to head_dim; up to 4 axes; tensors and weights 16-byte
+ * aligned, strides whole 16-byte vectors. */
+MZ_API int mz_qk_norm_rope(
+    void *q_out, int64_t q_out_tok_stride, int64_t q_out_head_stride, void *k_out,
+    int64_t k_out_tok_stride, int64_t k_out_head_stride, const void *q, int64_t q_tok_stride,
+    int64_t q_head_stride, const void *k, int64_t k_tok_stride, int64_t k_head_stride,
+    const void *v, int64_t v_tok_stride, int64_t v_head_stride, void *k_pool, void *v_pool,
+    const int64_t *slot_mapping, int32_t block_size, int64_t n_blocks, const int32_t *positions,
+    int64_t pos_axis_stride, int32_t n_axes, const float *inv_freq, const int32_t *freq_axes,
+    int32_t rot_dim, int32_t interleaved, const void *q_weight, const void *k_weight,
+    int32_t weight_dtype, float weight_offset, float eps, int32_t norm, int32_t n_tokens,
+    int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int32_t dtype, int32_t *dev_err,
+    mz_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
 /* Block-table gather.                                                       */
@@ -210,6 +280,68 @@ MZ_API int mz_paged_prefill(void *out, int32_t out_dtype, int64_t out_tok_stride
                             int32_t n_kv_heads, int32_t head_dim, int32_t block_size,
                             int64_t n_blocks, float scale, int32_t dtype, int32_t *dev_err,
                             mz_stream_t stream);
+
+/* Modified scores and masks, for the _mod entry points.  For a query token at
+ * position p of its sequence and a key at position t:
+ *   x = scale * q.k;  softcap > 0: x = softcap * tanh(x / softcap);
+ *   alibi_slopes: x -= alibi_slopes[query head] * |p - t|  (f32 [n_heads]);
+ *   the token sees the key iff  t < prefix  or
+ *     (t <= p  and  (t >= max(first, p - window + 1)  or  t < sink_tokens)),
+ * with prefix = prefix_lens[sequence] (NULL: 0; at most the sequence's length),
+ * window 0 for no window, and first = first_keys[sequence] in the decode calls,
+ * first_keys[row of q] in mz_paged_prefill_mod (NULL: 0; the document mask: the
+ * position at which the token's document starts).  A token that sees no key
+ * gets zeros.  Blocks that no token of the call sees are not read: their
+ * table entries may be stale.  All arrays are on the device.  Same
+ * place in the reference as the unmodified calls: the scaled dot product
+ * attention of src/mlxz/paged_attention/attention.py:40-42, whose models mask
+ * and cap; streaming_sink_size of src/mlxz/config.py:28-36 is sink_tokens. */
+typedef struct mz_score_mod {
+  float softcap;
+  int32_t window;
+  int32_t sink_tokens;
+  const float *alibi_slopes;
+  const int32_t *prefix_lens;
+  const int32_t *first_keys;
+} mz_score_mod;
+
+/* mz_paged_decode with modified scores and masks.  Unlike there, n_q_tokens > 1
+ * tokens are the sequence's last ones (drafted tokens, their K/V appended):
+ * token i is at position ctx_lens[b] - n_q_tokens + i (below 0: zeros).
+ * Arguments and rules otherwise as mz_paged_decode. */
+MZ_API int mz_paged_decode_mod(void *out, int32_t out_dtype, int64_t out_seq_stride,
+                               int64_t out_tok_stride, int64_t out_head_stride, const void *q,
+                               int64_t q_seq_stride, int64_t q_tok_stride, int64_t q_head_stride,
+                               int32_t n_q_tokens, const void *k_pool, const void *v_pool,
+                               const int32_t *block_tables, int32_t max_blocks_per_seq,
+                               const int32_t *ctx_lens, int32_t n_seqs, int32_t n_heads,
+                               int32_t n_kv_heads, int32_t head_dim, int32_t block_size,
+                               int64_t n_blocks, float scale, const mz_score_mod *mod,
+                               int32_t dtype, int32_t num_warps, void *workspace,
+                               size_t workspace_bytes, int32_t *dev_err, mz_stream_t stream);
+
+/* mz_paged_append_decode_ex with modified scores and masks. */
+MZ_API int mz_paged_append_decode_mod(
+    void *out, int32_t out_dtype, int64_t out_seq_stride, int64_t out_head_stride, const void *q,
+    int64_t q_seq_stride, int64_t q_head_stride, void *k_pool, void *v_pool, const void *k_new,
+    const void *v_new, int64_t new_seq_stride, int64_t new_head_stride,
+    const int32_t *block_tables, int32_t max_blocks_per_seq, const int32_t *ctx_lens,
+    int32_t n_seqs, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int32_t block_size,
+    int64_t n_blocks, float scale, const mz_score_mod *mod, int32_t dtype, int32_t num_warps,
+    uint32_t flags, void *workspace, size_t workspace_bytes, int32_t *dev_err,
+    mz_stream_t stream);
+
+/* mz_paged_prefill with modified scores and masks (first_keys per row of q). */
+MZ_API int mz_paged_prefill_mod(void *out, int32_t out_dtype, int64_t out_tok_stride,
+                                int64_t out_head_stride, const void *q, int64_t q_tok_stride,
+                                int64_t q_head_stride, int32_t n_rows, const int32_t *q_start,
+                                const int32_t *q_len, int32_t max_q_len, const void *k_pool,
+                                const void *v_pool, const int32_t *block_tables,
+                                int32_t max_blocks_per_seq, const int32_t *ctx_lens,
+                                int32_t n_seqs, int32_t n_heads, int32_t n_kv_heads,
+                                int32_t head_dim, int32_t block_size, int64_t n_blocks,
+                                float scale, const mz_score_mod *mod, int32_t dtype,
+                                int32_t *dev_err, mz_stream_t stream);
 
 /* Launch flags of the _ex / allgather entry points.
  * MZ_LAUNCH_OVERLAP_PREVIOUS: the launch may begin while the kernel ahead of it

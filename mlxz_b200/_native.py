@@ -31,6 +31,8 @@ MZ_DEVERR_SLOT = 2
 MZ_DEVERR_CONTEXT = 4
 MZ_DEVERR_TIMEOUT = 8
 MZ_DEVERR_ROWS = 16
+MZ_DEVERR_BLOCKS = 32
+MZ_DEVERR_AXIS = 64
 
 _DEVERR_NAMES = {
     MZ_DEVERR_BLOCK_ID: "block id out of range",
@@ -38,6 +40,8 @@ _DEVERR_NAMES = {
     MZ_DEVERR_CONTEXT: "context length out of range",
     MZ_DEVERR_TIMEOUT: "bounded wait timed out",
     MZ_DEVERR_ROWS: "query rows out of range",
+    MZ_DEVERR_BLOCKS: "more new blocks needed than given",
+    MZ_DEVERR_AXIS: "position axis out of range",
 }
 
 
@@ -85,6 +89,14 @@ class PeerOutputs(ctypes.Structure):
                 ("arrivals", ctypes.c_void_p), ("epoch", ctypes.c_uint32)]
 
 
+class ScoreMod(ctypes.Structure):
+    """mz_score_mod: modified scores and masks of an attention call."""
+
+    _fields_ = [("softcap", ctypes.c_float), ("window", ctypes.c_int32),
+                ("sink_tokens", ctypes.c_int32), ("alibi_slopes", ctypes.c_void_p),
+                ("prefix_lens", ctypes.c_void_p), ("first_keys", ctypes.c_void_p)]
+
+
 # name -> argtypes (every function returns int32 status)
 _SIGNATURES: dict[str, list] = {
     "mz_abi_version": [],
@@ -95,6 +107,12 @@ _SIGNATURES: dict[str, list] = {
                            _i32, _i64, _i32, _vp, _vp],
     "mz_kv_gather": [_vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _i32, _i64, _i32, _i32, _i32,
                      _i64, _i32, _vp, _vp],
+    "mz_paged_plan": [_vp, _i32, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32, _i64, _vp, _vp, _vp,
+                      _vp, _vp, _vp, _vp, _vp],
+    "mz_qk_norm_rope": [_vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp,
+                        _i64, _i64, _vp, _vp, _vp, _i32, _i64, _vp, _i64, _i32, _vp, _vp, _i32,
+                        _i32, _vp, _vp, _i32, _f32, _f32, _i32, _i32, _i32, _i32, _i32, _i32,
+                        _vp, _vp],
     "mz_paged_decode_workspace_size": [_i32, _i32, _i32, _i32, _i32, _i32,
                                        ctypes.POINTER(_sz)],
     "mz_paged_decode_workspace_size_ex": [_i32, _i32, _i32, _i32, _i32, _i32, _i32,
@@ -102,12 +120,19 @@ _SIGNATURES: dict[str, list] = {
     "mz_paged_decode": [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _vp,
                         _vp, _i32, _vp, _i32, _i32, _i32, _i32, _i32, _i64, _f32, _i32, _i32,
                         _vp, _sz, _vp, _vp],
+    "mz_paged_decode_mod": [_vp, _i32, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _i32, _vp, _vp,
+                            _vp, _i32, _vp, _i32, _i32, _i32, _i32, _i32, _i64, _f32,
+                            ctypes.POINTER(ScoreMod), _i32, _i32, _vp, _sz, _vp, _vp],
     "mz_paged_append_decode": [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64,
                                _i64, _vp, _i32, _vp, _i32, _i32, _i32, _i32, _i32, _i64, _f32,
                                _i32, _i32, _vp, _sz, _vp, _vp],
     "mz_paged_append_decode_ex": [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp,
                                   _i64, _i64, _vp, _i32, _vp, _i32, _i32, _i32, _i32, _i32,
                                   _i64, _f32, _i32, _i32, ctypes.c_uint32, _vp, _sz, _vp, _vp],
+    "mz_paged_append_decode_mod": [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp,
+                                   _i64, _i64, _vp, _i32, _vp, _i32, _i32, _i32, _i32, _i32,
+                                   _i64, _f32, ctypes.POINTER(ScoreMod), _i32, _i32,
+                                   ctypes.c_uint32, _vp, _sz, _vp, _vp],
     "mz_paged_append_decode_allgather": [ctypes.POINTER(PeerOutputs), _i32, _i64, _i64, _vp,
                                          _i64, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _i32,
                                          _vp, _i32, _i32, _i32, _i32, _i32, _i64, _f32, _i32,
@@ -117,6 +142,9 @@ _SIGNATURES: dict[str, list] = {
                              _i32, _i32, _i64, _i32, _vp, _vp],
     "mz_paged_prefill": [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _i32, _vp, _vp, _vp,
                          _i32, _vp, _i32, _i32, _i32, _i32, _i32, _i64, _f32, _i32, _vp, _vp],
+    "mz_paged_prefill_mod": [_vp, _i32, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _vp, _i32, _vp,
+                             _vp, _vp, _i32, _vp, _i32, _i32, _i32, _i32, _i32, _i64, _f32,
+                             ctypes.POINTER(ScoreMod), _i32, _vp, _vp],
     "mz_ipc_export": [_vp, _vp, ctypes.POINTER(ctypes.c_uint64)],
     "mz_ipc_open": [_vp, ctypes.c_uint64, ctypes.POINTER(_vp), ctypes.POINTER(_vp)],
     "mz_ipc_close": [_vp],

@@ -28,6 +28,7 @@
 #include <mutex>
 
 #include "common.cuh"
+#include "score_mod.cuh"
 
 namespace mz {
 namespace decode {
@@ -92,6 +93,12 @@ struct Params {
   uint32_t wait_epoch = 0;  // 0: no folded wait
 };
 
+// The same with modified scores and masks (score_mod.cuh); query token i of
+// n_q sits at position ctx - n_q + i.
+struct ModParams : Params {
+  ScoreMod mod;
+};
+
 struct Cursor {
   int b, h, t, n, ctx;
   int pos;
@@ -115,7 +122,46 @@ __device__ __forceinline__ int clamped_ctx(const Params &p, int b) {
   return c;
 }
 
-__device__ __forceinline__ void advance(Cursor &c, const Params &p) {
+// Tiles of sequence b that its rows read: all of them, or with ModParams those
+// that the window leaves.  A cursor's t counts these; its ctx stays the
+// sequence's own.
+__device__ __forceinline__ int span_tiles(const Params &, int, int ctx) { return ntiles_of(ctx); }
+
+// What sequence b's mask leaves: keys [0, head) in any case, then those from lo
+// (the first query token's; later ones' are no lower) on.
+struct MaskSpan {
+  int prefix, head, lo;
+};
+
+__device__ __forceinline__ MaskSpan mask_span(const ModParams &p, int b, int ctx) {
+  MaskSpan s;
+  s.prefix = p.mod.prefix ? max(0, min(p.mod.prefix[b], ctx)) : 0;
+  s.head = max(s.prefix, p.mod.sink);
+  s.lo = p.mod.first ? max(0, p.mod.first[b]) : 0;
+  if (p.mod.window > 0) s.lo = max(s.lo, ctx - p.n_q - p.mod.window + 1);
+  return s;
+}
+
+// Tiles between the head's last and the one that holds lo (or the last tile,
+// which is read in any case) are left out.
+__device__ __forceinline__ int span_tiles(const ModParams &p, int b, int ctx) {
+  const int n = ntiles_of(ctx);
+  if (n == 0) return 0;
+  const MaskSpan s = mask_span(p, b, ctx);
+  const int skip = min(s.lo, ctx - 1) / kTileTok - ntiles_of(s.head);
+  return skip > 0 ? n - skip : n;
+}
+
+// The sequence's own tile that a cursor's tile t stands for.
+__device__ __forceinline__ int own_tile(const Params &, int, int t, int, int) { return t; }
+__device__ __forceinline__ int own_tile(const ModParams &p, int b, int t, int n, int ctx) {
+  const int skip = ntiles_of(ctx) - n;
+  if (skip == 0) return t;
+  return t < ntiles_of(mask_span(p, b, ctx).head) ? t : t + skip;
+}
+
+template <class P>
+__device__ __forceinline__ void advance(Cursor &c, const P &p) {
   ++c.pos;
   if (++c.t == c.n) {
     c.t = 0;
@@ -127,7 +173,7 @@ __device__ __forceinline__ void advance(Cursor &c, const Params &p) {
           break;
         }
         c.ctx = clamped_ctx(p, c.b);
-        c.n = ntiles_of(c.ctx);
+        c.n = span_tiles(p, c.b, c.ctx);
         if (c.n > 0) break;
       }
     }
@@ -135,11 +181,12 @@ __device__ __forceinline__ void advance(Cursor &c, const Params &p) {
 }
 
 // Cursor at flat tile x (0 <= x < T), found with a warp scan over sequences.
-__device__ __forceinline__ Cursor locate(const Params &p, int x, int lane) {
+template <class P>
+__device__ __forceinline__ Cursor locate(const P &p, int x, int lane) {
   int base = 0, bf = 0;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     const int b = b0 + lane;
-    const int c = (b < p.B) ? ntiles_of(clamped_ctx(p, b)) * p.Hkv : 0;
+    const int c = (b < p.B) ? span_tiles(p, b, clamped_ctx(p, b)) * p.Hkv : 0;
     int incl = c;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -158,7 +205,7 @@ __device__ __forceinline__ Cursor locate(const Params &p, int x, int lane) {
   Cursor cur;
   cur.b = bf;
   cur.ctx = clamped_ctx(p, bf);
-  cur.n = ntiles_of(cur.ctx);
+  cur.n = span_tiles(p, bf, cur.ctx);
   const int r = x - base;
   cur.h = r / cur.n;
   cur.t = r - cur.h * cur.n;
@@ -308,14 +355,15 @@ struct Sched {
   bool p_done, static_taken;
 
   // Returns false (nothing to do, no counter touched) when T == 0.
-  __device__ bool init(const Params &p, int lane_, int wid_, int W_, Unit *uq_) {
+  template <class P>
+  __device__ bool init(const P &p, int lane_, int wid_, int W_, Unit *uq_) {
     lane = lane_;
     wid = wid_;
     W = W_;
     uq = uq_;
     int t = 0, longest = 0;
     for (int b = lane; b < p.B; b += 32) {
-      const int n = ntiles_of(clamped_ctx(p, b));
+      const int n = span_tiles(p, b, clamped_ctx(p, b));
       t += n;
       longest = max(longest, n);
     }
@@ -336,7 +384,7 @@ struct Sched {
       // the batch
       int pc = 0;
       for (int b = lane; b < p.B; b += 32)
-        pc += (ntiles_of(clamped_ctx(p, b)) + kBiPieceTiles - 1) / kBiPieceTiles;
+        pc += (span_tiles(p, b, clamped_ctx(p, b)) + kBiPieceTiles - 1) / kBiPieceTiles;
 #pragma unroll
       for (int o = 16; o; o >>= 1) pc += __shfl_xor_sync(0xffffffffu, pc, o);
       per_s = 0;
@@ -373,7 +421,8 @@ struct Sched {
     return x < t_s ? x / per_s : W + (x - t_s) / chunk;
   }
 
-  __device__ bool next_unit(const Params &p) {
+  template <class P>
+  __device__ bool next_unit(const P &p) {
     int start = 0, end = 0, u = 0, fp = 0, np = 1;
     bool ok = false;
     if (!static_taken) {
@@ -408,7 +457,7 @@ struct Sched {
         int pbase = 0, tbase = 0, bf = 0;
         for (int b0 = 0; b0 < p.B; b0 += 32) {
           const int b = b0 + lane;
-          const int n = (b < p.B) ? ntiles_of(clamped_ctx(p, b)) : 0;
+          const int n = (b < p.B) ? span_tiles(p, b, clamped_ctx(p, b)) : 0;
           const int pc = p.Hkv * ((n + kBiPieceTiles - 1) / kBiPieceTiles);
           int ip = pc, it = n;
 #pragma unroll
@@ -431,7 +480,7 @@ struct Sched {
           pbase += __shfl_sync(0xffffffffu, ip, 31);
           tbase += __shfl_sync(0xffffffffu, it, 31);
         }
-        const int n = ntiles_of(clamped_ctx(p, bf));
+        const int n = span_tiles(p, bf, clamped_ctx(p, bf));
         np = (n + kBiPieceTiles - 1) / kBiPieceTiles;
         const int r = tk - pbase;
         const int h = r / np, j = r - (r / np) * np;
@@ -451,7 +500,8 @@ struct Sched {
   }
 
   // Cursor at the unit's first tile; the unit descriptor goes to the ring.
-  __device__ __forceinline__ void push_unit(const Params &p, int start, int end, int u,
+  template <class P>
+  __device__ __forceinline__ void push_unit(const P &p, int start, int end, int u,
                                             int fp = 0, int np = 1) {
     pc = locate(p, start, lane);
     if (lane == 0) {
@@ -476,8 +526,8 @@ struct Sched {
   // launch): start the copies of the first (up to S) tiles of this warp's
   // static share.  Reads only ctx, the block tables and the pools (through
   // locate and issue); no ticket, no workspace word.
-  template <int S, class IssueFn>
-  __device__ __forceinline__ void prefetch_static(const Params &p, IssueFn &&issue) {
+  template <int S, class P, class IssueFn>
+  __device__ __forceinline__ void prefetch_static(const P &p, IssueFn &&issue) {
     if (static_taken) return;
     static_taken = true;
     if (!(per_s > 0 && (int64_t)wid * per_s < t_s)) return;
@@ -493,8 +543,8 @@ struct Sched {
   }
 
   // Keep S tiles in flight; issue(stage, cursor) starts one tile's copies.
-  template <int S, class IssueFn>
-  __device__ __forceinline__ void refill(const Params &p, int consumed, IssueFn &&issue) {
+  template <int S, class P, class IssueFn>
+  __device__ __forceinline__ void refill(const P &p, int consumed, IssueFn &&issue) {
     while (!p_done && issued - consumed < S) {
       if (p_left == 0 && !next_unit(p)) {
         p_done = true;
@@ -578,6 +628,9 @@ __device__ __forceinline__ void merge_piece(float &M, float &Ls, float4 &acc, fl
   M = Mn;
 }
 
+// 1 / (row sum); a row whose mask left no key has sum 0 and O = 0, its output.
+__device__ __forceinline__ float row_inverse(float sum) { return sum == 0.f ? 0.f : 1.f / sum; }
+
 // Merge straight from global memory: the pieces are read four at a time, all
 // four loads in flight before the combine that needs them.
 template <int D, bool GATHER>
@@ -606,7 +659,7 @@ __device__ __forceinline__ void merge_global(const Params &p, int b, int h, int 
       for (int j = 0; j < 4; ++j)
         if (k0 + j < nparts) merge_piece(M, Ls, acc, mlk[j], ok[j]);
     }
-    const float inv = 1.f / Ls;
+    const float inv = row_inverse(Ls);
     const int64_t o = row_offset(p.o_sb, p.o_st, p.o_sh, b, h, r, p.G) + d;
     store_pair(p, o, acc.x * inv, acc.y * inv);
     store_pair(p, o + 2, acc.z * inv, acc.w * inv);
@@ -678,7 +731,7 @@ __device__ __forceinline__ void merge_staged(const Params &p, int b, int h, int 
     const int e = 4 * lane + 128 * it;
     if (e < E) {
       const int r = e / D, d = e - r * D;
-      const float inv = 1.f / Ls[it];
+      const float inv = row_inverse(Ls[it]);
       const int64_t o = row_offset(p.o_sb, p.o_st, p.o_sh, b, h, r, p.G) + d;
       store_pair(p, o, acc[it].x * inv, acc[it].y * inv);
       store_pair(p, o + 2, acc[it].z * inv, acc[it].w * inv);

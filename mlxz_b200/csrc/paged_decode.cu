@@ -22,6 +22,8 @@
 // us static, 237 us with 15 % in 9-tile chunks: every chunk adds a piece to
 // merge), so the default hands out everything statically; merges of split
 // pairs are deferred to the end of each warp's loop.
+#include <type_traits>
+
 #include "decode_common.cuh"
 
 #ifndef MZ_DECODE_STAGES_D128
@@ -43,9 +45,11 @@ struct Cfg {
   static constexpr int kSmemBytes = kSmemTiles + kSmemBars + kSmemUnits + kSmemDefer + 1024;
 };
 
-template <int D, bool BF16, bool GATHER>
+// P: Params, or ModParams for modified scores and masks.
+template <int D, bool BF16, bool GATHER, class P>
 __device__ __forceinline__ void decode_tiles(const CUtensorMap &tmK, const CUtensorMap &tmV,
-                                             const Params &p) {
+                                             const P &p) {
+  constexpr bool MOD = std::is_same<P, ModParams>::value;
   using C = Cfg<D>;
   constexpr int S = C::kStages;
   constexpr int KS = D / 16;  // k-steps of Q.K^T, also n-tile pairs of P.V
@@ -80,12 +84,13 @@ __device__ __forceinline__ void decode_tiles(const CUtensorMap &tmK, const CUten
   const uint64_t pol = l2_policy_evict_first();
   auto issue = [&](int s, const Cursor &c) {
     if (lane == 0) {
-      int32_t blk = p.tables[(int64_t)c.b * p.max_blocks + c.t / p.tpb];
+      const int t = own_tile(p, c.b, c.t, c.n, c.ctx);
+      int32_t blk = p.tables[(int64_t)c.b * p.max_blocks + t / p.tpb];
       if (blk < 0 || blk >= p.n_blocks) {
         dev_error(p.err, MZ_DEVERR_BLOCK_ID);
         blk = 0;
       }
-      const int y = static_cast<int>(((int64_t)blk * p.Hkv + c.h) * p.bs + (c.t % p.tpb) * kTileTok);
+      const int y = static_cast<int>(((int64_t)blk * p.Hkv + c.h) * p.bs + (t % p.tpb) * kTileTok);
       const uint32_t bar = bar0 + 8 * s;
       const uint32_t dk = stage0 + s * C::kStageBytes;
       mbar_arrive_expect_tx(bar, C::kStageBytes);
@@ -110,6 +115,10 @@ __device__ __forceinline__ void decode_tiles(const CUtensorMap &tmK, const CUten
 
   UnitReader ur;
   bool seg_first = true;
+  // MOD: the piece's mask, and the positions, lower ends and slopes of rows g, g + 8
+  MaskSpan span{};
+  int skip = 0, p_min = 0, lo_max = 0, pos0 = 0, pos1 = 0, lo0 = 0, lo1 = 0;
+  float slope0 = 0.f, slope1 = 0.f;
 
   // Until the launch ahead has completed (programmatic dependent launch) only
   // ctx, the tables and the pools are read: the first tiles of the static
@@ -133,8 +142,25 @@ __device__ __forceinline__ void decode_tiles(const CUtensorMap &tmK, const CUten
     if (seg_first || cc.t == 0) {
       // New piece: load the grouped query rows as A fragments.
       seg_first = false;
-      m0 = m1 = -INFINITY;
+      m0 = m1 = MOD ? kNoMax : -INFINITY;
       l0 = l1 = 0.f;
+      if constexpr (MOD) {
+        span = mask_span(p, cc.b, cc.ctx);
+        skip = ntiles_of(cc.ctx) - cc.n;
+        p_min = cc.ctx - p.n_q;
+        pos0 = p_min + g / p.G;
+        pos1 = p_min + (g + 8) / p.G;
+        // lower ends rise with the token where the window sets them
+        const int first = p.mod.first ? max(0, p.mod.first[cc.b]) : 0;
+        const int w = p.mod.window > 0 ? p.mod.window : 1 << 30;
+        lo0 = max(first, pos0 - w + 1);
+        lo1 = max(first, pos1 - w + 1);
+        lo_max = max(first, cc.ctx - w);
+        if (p.mod.slopes) {
+          slope0 = g < p.rows ? p.mod.slopes[cc.h * p.G + g % p.G] * kLog2e : 0.f;
+          slope1 = g + 8 < p.rows ? p.mod.slopes[cc.h * p.G + (g + 8) % p.G] * kLog2e : 0.f;
+        }
+      }
 #pragma unroll
       for (int n = 0; n < NT; ++n) oacc[n][0] = oacc[n][1] = oacc[n][2] = oacc[n][3] = 0.f;
       const auto *q16 = static_cast<const uint16_t *>(p.q);
@@ -160,7 +186,9 @@ __device__ __forceinline__ void decode_tiles(const CUtensorMap &tmK, const CUten
     uint8_t *vt = kt + C::kTileBytes;
     const uint32_t kb = stage0 + s * C::kStageBytes;
     const uint32_t vb = kb + C::kTileBytes;
-    const int nvalid = min(kTileTok, cc.ctx - cc.t * kTileTok);
+    const int tile = MOD && cc.t >= ntiles_of(span.head) ? cc.t + skip : cc.t;  // own_tile
+    const int key0 = tile * kTileTok;
+    const int nvalid = min(kTileTok, cc.ctx - key0);
     const bool last_tile = (cc.t == cc.n - 1);
     if (p.kn != nullptr && last_tile) {
       // Fused append: the sequence's new token is its last attended one.  Write
@@ -184,7 +212,15 @@ __device__ __forceinline__ void decode_tiles(const CUtensorMap &tmK, const CUten
       }
       __syncwarp();
     }
-    if (nvalid < kTileTok) {
+    if (MOD && key0 < span.lo && key0 + kTileTok > span.head) {
+      // Keys that no row sees may hold anything: exact zeros for V here too.
+      for (int e = lane; e < kTileTok * (D / 8); e += 32) {
+        const int tok = e / (D / 8), d = (e % (D / 8)) * 8, key = key0 + tok;
+        if (key >= cc.ctx || (key < span.lo && key >= span.head))
+          *reinterpret_cast<uint4 *>(vt + swz128(tok, 2 * d)) = make_uint4(0, 0, 0, 0);
+      }
+      __syncwarp();
+    } else if (nvalid < kTileTok) {
       // Rows past the context may hold stale data; make them exact zeros so
       // that 0 * V stays 0 in P.V.
       for (int e = lane; e < (kTileTok - nvalid) * (D / 8); e += 32) {
@@ -208,13 +244,25 @@ __device__ __forceinline__ void decode_tiles(const CUtensorMap &tmK, const CUten
 
     // Online softmax (exp2 domain), rows g (regs 0,1) and g+8 (regs 2,3).
     float mx0 = -INFINITY, mx1 = -INFINITY;
+    // MOD: every row sees every key of the tile
+    const bool all_seen = MOD && key0 >= lo_max && key0 + kTileTok - 1 <= p_min;
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int tok = n * 8 + 2 * cq + (e & 1);
         float x = sacc[n][e] * p.scale_log2;
-        if (tok >= nvalid) x = -INFINITY;
+        if constexpr (MOD) {
+          const int key = key0 + tok, pos = e < 2 ? pos0 : pos1, lo = e < 2 ? lo0 : lo1;
+          if (p.mod.z_scale != 0.f) x = p.mod.cap_log2 * tanh_mod(sacc[n][e] * p.mod.z_scale);
+          if (p.mod.slopes)
+            x = fmaf(-(e < 2 ? slope0 : slope1), fabsf(static_cast<float>(pos - key)), x);
+          if (!all_seen && !(key < span.prefix ||
+                             (key <= pos && (key >= lo || key < p.mod.sink))))
+            x = -INFINITY;
+        } else {
+          if (tok >= nvalid) x = -INFINITY;
+        }
         sacc[n][e] = x;
         if (e < 2) mx0 = fmaxf(mx0, x); else mx1 = fmaxf(mx1, x);
       }
@@ -304,7 +352,8 @@ __device__ __forceinline__ void decode_tiles(const CUtensorMap &tmK, const CUten
       const int uf = p.batch_invariant ? sch.W + ur.fp : sch.unit_of(pbh);
       const int ul = p.batch_invariant ? uf + ur.np - 1 : sch.unit_of(pbh + cc.n - 1);
       if (uf == ul) {
-        const float i0 = 1.f / L0, i1 = two_groups ? 1.f / L1 : 0.f;
+        const float i0 = MOD ? row_inverse(L0) : 1.f / L0;
+        const float i1 = !two_groups ? 0.f : MOD ? row_inverse(L1) : 1.f / L1;
         if (g < p.rows) {
           const int64_t o = row_offset(p.o_sb, p.o_st, p.o_sh, cc.b, cc.h, g, p.G);
 #pragma unroll
@@ -357,6 +406,15 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
   decode_tiles<D, BF16, false>(tmK, tmV, p);
 }
 
+// Modified scores and masks (score_mod.cuh).
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kWarps * 32, 2)
+    paged_decode_mod_kernel(const __grid_constant__ CUtensorMap tmK,
+                            const __grid_constant__ CUtensorMap tmV, const ModParams p) {
+  launch_dependents();
+  decode_tiles<D, BF16, false>(tmK, tmV, p);
+}
+
 // The all-gather instantiation: every output store also goes to the peers'
 // buffers, and the grid's last block signals them.
 template <int D, bool BF16>
@@ -392,6 +450,13 @@ int gather_smem_attr() {
   static DeviceOnce once;
   return smem_optin(paged_decode_gather_kernel<D, BF16>, Cfg<D>::kSmemBytes, once,
                     "setting the all-gather kernel's shared memory");
+}
+
+template <int D, bool BF16>
+int mod_smem_attr() {
+  static DeviceOnce once;
+  return smem_optin(paged_decode_mod_kernel<D, BF16>, Cfg<D>::kSmemBytes, once,
+                    "setting the modified-score kernel's shared memory");
 }
 
 int ctas_per_sm(int D, bool bf16, int *out) {
@@ -440,6 +505,7 @@ struct DecodeArgs {
   cudaStream_t stream;
   const mz_peer_outputs *peers = nullptr;  // all-gather over peer memory, or none
   uint32_t flags = 0;                      // MZ_LAUNCH_*
+  const mz_score_mod *mod = nullptr;       // modified scores and masks, or none
 };
 
 // The most pieces a batch-invariant launch cuts: every pair at full capacity.
@@ -585,6 +651,12 @@ int launch(const DecodeArgs &a, int64_t warps, const WsLayout &ws, void *scratch
     }
   }
 
+  ModParams mp;
+  if (a.mod) {
+    static_cast<Params &>(mp) = p;
+    if (int rc = make_score_mod(&mp.mod, a.mod, a.scale, (int64_t)a.max_blocks * a.bs, fn)) return rc;
+  }
+
   int per_sm = 0;  // also sets the kernel's shared-memory attribute (once)
   if (int rc = ctas_per_sm(a.D, bf16, &per_sm)) return rc;
   if (clear_counters) {
@@ -605,7 +677,10 @@ int launch(const DecodeArgs &a, int64_t warps, const WsLayout &ws, void *scratch
 #define MZ_LAUNCH(D_, BF_)                                                          \
   do {                                                                              \
     cfg.dynamicSmemBytes = Cfg<D_>::kSmemBytes;                                     \
-    if (a.peers) {                                                                  \
+    if (a.mod) {                                                                    \
+      if (int rc = mod_smem_attr<D_, BF_>()) return rc;                             \
+      le = cudaLaunchKernelEx(&cfg, paged_decode_mod_kernel<D_, BF_>, tk, tv, mp);  \
+    } else if (a.peers) {                                                           \
       if (int rc = gather_smem_attr<D_, BF_>()) return rc;                          \
       le = cudaLaunchKernelEx(&cfg, paged_decode_gather_kernel<D_, BF_>, tk, tv, p); \
     } else {                                                                        \
@@ -742,7 +817,8 @@ static int append_decode(void *out, int32_t out_dtype, int64_t out_seq_stride,
                          int32_t n_kv_heads, int32_t head_dim, int32_t block_size,
                          int64_t n_blocks, float scale, int32_t dtype, int32_t num_warps,
                          uint32_t flags, void *workspace, size_t workspace_bytes,
-                         int32_t *dev_err, mz_stream_t stream, const char *fn) {
+                         int32_t *dev_err, mz_stream_t stream, const char *fn,
+                         const mz_score_mod *mod = nullptr) {
   DecodeArgs a = make_args(out, out_dtype, out_seq_stride, 0, out_head_stride, q, q_seq_stride, 0,
                            q_head_stride, 1, k_pool, v_pool, block_tables, max_blocks_per_seq,
                            ctx_lens, n_seqs, n_heads, n_kv_heads, head_dim, block_size, n_blocks,
@@ -754,10 +830,42 @@ static int append_decode(void *out, int32_t out_dtype, int64_t out_seq_stride,
   if (flags & ~(MZ_LAUNCH_OVERLAP_PREVIOUS | MZ_DECODE_BATCH_INVARIANT))
     return fail(MZ_ERR_INVALID_ARG, "%s: unknown flags", fn);
   a.flags = flags;
+  a.mod = mod;
   if (!k_new || !v_new) return fail(MZ_ERR_INVALID_ARG, "%s: null k_new / v_new", fn);
   int64_t warps = 0;
   WsLayout ws;
   if (int rc = validate(a, fn, &warps, &ws)) return rc;
+  if (n_seqs == 0) return MZ_OK;
+  if (!workspace) return fail(MZ_ERR_WORKSPACE, "%s: workspace is null", fn);
+  if (workspace_bytes < ws.total)
+    return fail(MZ_ERR_WORKSPACE, "%s: workspace %zu bytes < required %zu", fn, workspace_bytes,
+                ws.total);
+  return launch(a, warps, ws, workspace, false, fn);
+}
+
+extern "C" int mz_paged_decode_mod(void *out, int32_t out_dtype, int64_t out_seq_stride,
+                                   int64_t out_tok_stride, int64_t out_head_stride, const void *q,
+                                   int64_t q_seq_stride, int64_t q_tok_stride,
+                                   int64_t q_head_stride, int32_t n_q_tokens, const void *k_pool,
+                                   const void *v_pool, const int32_t *block_tables,
+                                   int32_t max_blocks_per_seq, const int32_t *ctx_lens,
+                                   int32_t n_seqs, int32_t n_heads, int32_t n_kv_heads,
+                                   int32_t head_dim, int32_t block_size, int64_t n_blocks,
+                                   float scale, const mz_score_mod *mod, int32_t dtype,
+                                   int32_t num_warps, void *workspace, size_t workspace_bytes,
+                                   int32_t *dev_err, mz_stream_t stream) {
+  const char *fn = "mz_paged_decode_mod";
+  DecodeArgs a = make_args(out, out_dtype, out_seq_stride, out_tok_stride, out_head_stride, q,
+                           q_seq_stride, q_tok_stride, q_head_stride, n_q_tokens, k_pool, v_pool,
+                           block_tables, max_blocks_per_seq, ctx_lens, n_seqs, n_heads, n_kv_heads,
+                           head_dim, block_size, n_blocks, scale, dtype, num_warps, dev_err,
+                           stream);
+  int64_t warps = 0;
+  WsLayout ws;
+  if (int rc = validate(a, fn, &warps, &ws)) return rc;
+  ScoreMod sm;
+  if (int rc = make_score_mod(&sm, mod, scale, (int64_t)max_blocks_per_seq * block_size, fn)) return rc;
+  a.mod = mod;
   if (n_seqs == 0) return MZ_OK;
   if (!workspace) return fail(MZ_ERR_WORKSPACE, "%s: workspace is null", fn);
   if (workspace_bytes < ws.total)
@@ -796,6 +904,27 @@ extern "C" int mz_paged_append_decode_ex(
                        n_heads, n_kv_heads, head_dim, block_size, n_blocks, scale, dtype,
                        num_warps, flags, workspace, workspace_bytes, dev_err, stream,
                        "mz_paged_append_decode_ex");
+}
+
+extern "C" int mz_paged_append_decode_mod(
+    void *out, int32_t out_dtype, int64_t out_seq_stride, int64_t out_head_stride, const void *q,
+    int64_t q_seq_stride, int64_t q_head_stride, void *k_pool, void *v_pool, const void *k_new,
+    const void *v_new, int64_t new_seq_stride, int64_t new_head_stride,
+    const int32_t *block_tables, int32_t max_blocks_per_seq, const int32_t *ctx_lens,
+    int32_t n_seqs, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim, int32_t block_size,
+    int64_t n_blocks, float scale, const mz_score_mod *mod, int32_t dtype, int32_t num_warps,
+    uint32_t flags, void *workspace, size_t workspace_bytes, int32_t *dev_err,
+    mz_stream_t stream) {
+  const char *fn = "mz_paged_append_decode_mod";
+  if (n_seqs < 0 || max_blocks_per_seq <= 0 || block_size <= 0)
+    return fail(MZ_ERR_INVALID_ARG, "%s: bad sizes", fn);
+  ScoreMod sm;
+  if (int rc = make_score_mod(&sm, mod, scale, (int64_t)max_blocks_per_seq * block_size, fn)) return rc;
+  return append_decode(out, out_dtype, out_seq_stride, out_head_stride, q, q_seq_stride,
+                       q_head_stride, k_pool, v_pool, k_new, v_new, new_seq_stride,
+                       new_head_stride, block_tables, max_blocks_per_seq, ctx_lens, n_seqs,
+                       n_heads, n_kv_heads, head_dim, block_size, n_blocks, scale, dtype,
+                       num_warps, flags, workspace, workspace_bytes, dev_err, stream, fn, mod);
 }
 
 extern "C" int mz_paged_append_decode_allgather(

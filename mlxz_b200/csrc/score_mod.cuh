@@ -1,0 +1,71 @@
+// Scores beyond scaled products, and masks beyond the causal one, shared by
+// the decode and the prefill attention kernels.
+//
+// For a token at position p of a sequence and a key at position t,
+//   x = scale q.k;   x <- cap tanh(x / cap);   x <- x - slope_h |p - t|
+// and the key is seen iff
+//   t < prefix_b  or  (t <= p  and  (t >= lo  or  t < sink)),
+//   lo = max(first, p - window + 1).
+// A row that sees no key has output 0.  The kernels keep x in units of log2 e,
+// so that its exponential is one ex2.
+#pragma once
+
+#include <cmath>
+
+#include "common.cuh"
+
+namespace mz {
+
+struct ScoreMod {
+  const float *slopes;    // [n_heads], null: none
+  const int32_t *first;   // per sequence (decode) or per row (prefill), null: 0
+  const int32_t *prefix;  // per sequence, null: 0
+  int window;             // 0: none
+  int sink;
+  float z_scale;   // scale / cap; 0: no cap
+  float cap_log2;  // cap * log2(e)
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+// Running maximum of a row that has seen no key yet: finite, so that the
+// difference of two of them is 0 and not NaN, and below every score.
+constexpr float kNoMax = -3.0e38f;
+
+// tanh to a relative error of about 1e-6: the odd series to z^9 below 0.3 (its
+// next term is 5e-8 of z there), 1 - 2 / (e^(2 |z|) + 1) from there on, where
+// the subtraction loses no more than two bits.
+__device__ __forceinline__ float tanh_mod(float z) {
+  const float a = fabsf(z), z2 = z * z;
+  float s = fmaf(z2, 2.18694885e-2f, -5.39682540e-2f);
+  s = fmaf(s, z2, 1.33333333e-1f);
+  s = fmaf(s, z2, -3.33333333e-1f);
+  s = fmaf(s * z2, z, z);
+  const float e = fast_exp2(a * (2.f * kLog2e));
+  const float t = copysignf(1.f - __fdividef(2.f, e + 1.f), z);
+  return a < 0.3f ? s : t;
+}
+
+// Host side: the fields of mz_score_mod checked and folded with the scale.
+// `tokens`: the table's capacity, which bounds what window and sink can mean.
+inline int make_score_mod(ScoreMod *m, const mz_score_mod *mod, float scale, int64_t tokens,
+                          const char *fn) {
+  if (!mod) return fail(MZ_ERR_INVALID_ARG, "%s: mod is null", fn);
+  if (!std::isfinite(mod->softcap) || mod->softcap < 0.f)
+    return fail(MZ_ERR_INVALID_ARG, "%s: softcap must be finite and not negative", fn);
+  if (mod->window < 0 || mod->sink_tokens < 0)
+    return fail(MZ_ERR_INVALID_ARG, "%s: window and sink_tokens must not be negative", fn);
+  const void *ptrs[] = {mod->alibi_slopes, mod->prefix_lens, mod->first_keys};
+  for (const void *x : ptrs)
+    if (!aligned(x, 4)) return fail(MZ_ERR_ALIGNMENT, "%s: mod arrays need 4-byte alignment", fn);
+  m->slopes = mod->alibi_slopes;
+  m->first = mod->first_keys;
+  m->prefix = mod->prefix_lens;
+  // a window of the whole table hides nothing; no position exceeds it either
+  m->window = mod->window >= tokens ? 0 : mod->window;
+  m->sink = static_cast<int>(mod->sink_tokens < tokens ? mod->sink_tokens : tokens);
+  m->z_scale = mod->softcap > 0.f ? scale / mod->softcap : 0.f;
+  m->cap_log2 = static_cast<float>(static_cast<double>(mod->softcap) * 1.4426950408889634);
+  return MZ_OK;
+}
+
+}  // namespace mz

@@ -12,6 +12,7 @@ import ctypes
 import math
 import os
 from collections import OrderedDict
+from typing import NamedTuple
 
 import torch
 
@@ -94,6 +95,17 @@ def _after(device: int) -> None:
 
 def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
+
+
+def _call(device: int, name: str, *args) -> None:
+    """nat.call with ``device`` current: a launch goes to the current device,
+    which need not be the tensors' own."""
+    if torch.cuda.current_device() == device:
+        nat.call(name, *args, error_word(device).data_ptr(), _stream(device))
+    else:
+        with torch.cuda.device(device):
+            nat.call(name, *args, error_word(device).data_ptr(), _stream(device))
+    _after(device)
 
 
 def _check_pools(k_pool: torch.Tensor, v_pool: torch.Tensor) -> tuple[int, int, int, int]:
@@ -212,6 +224,179 @@ def kv_gather(k_pool: torch.Tensor, v_pool: torch.Tensor, block_tables: torch.Te
 
 
 # ---------------------------------------------------------------------------
+# Step metadata
+# ---------------------------------------------------------------------------
+
+class PagedPlan(NamedTuple):
+    """What ``paged_plan`` builds for one step of B sequences and n_rows rows."""
+
+    q_start: torch.Tensor    # int32 [B], first row of each sequence
+    positions: torch.Tensor  # int32 [n_rows], position of each row's token
+    slots: torch.Tensor      # int64 [n_rows], its pool slot (-1 behind the last sequence)
+    lengths: torch.Tensor    # int32 [B], cached tokens with the new ones
+    held: torch.Tensor       # int32 [B], blocks in each table
+    n_new: torch.Tensor      # int32 [1], new blocks needed
+
+
+def paged_plan(block_tables: torch.Tensor, ctx_lens: torch.Tensor, q_lens: torch.Tensor,
+               n_rows: int, block_size: int, n_blocks: int, new_ids: torch.Tensor | None = None,
+               held: torch.Tensor | None = None) -> PagedPlan:
+    """Block tables, slot map and positions of a step, from the sequences'
+    lengths, in one launch (mz_paged_plan).
+
+    Sequence b has ``ctx_lens[b]`` cached tokens in ``held[b]`` blocks (default
+    ``ceil(ctx / block_size)``) of ``block_tables[b]`` and gets ``q_lens[b]``
+    new ones.  Blocks that it lacks are taken from ``new_ids`` in order,
+    sequence by sequence (``BlockManager.allocate``'s order), and written into
+    ``block_tables`` in place.  ``n_rows`` >= ``sum(q_lens)``; rows behind the
+    last sequence get slot -1 (skipped by the appends) and position 0.
+    ``n_blocks``: blocks of the pools (bounds the ids)."""
+    if block_tables.dim() != 2:
+        raise ValueError("block_tables must be [B, max_blocks]")
+    device = block_tables.device
+    _as_i32(block_tables, device, "block_tables")
+    B, width = block_tables.shape
+    for t, name in ((ctx_lens, "ctx_lens"), (q_lens, "q_lens"), (held, "held")):
+        if t is not None:
+            _as_i32(t, device, name)
+            if t.numel() != B:
+                raise ValueError(f"{name} must hold one entry per sequence ({B})")
+    if new_ids is not None:
+        _as_i32(new_ids, device, "new_ids")
+    if n_rows < 0 or block_size < 1 or n_blocks < 1:
+        raise ValueError("n_rows must be >= 0, block_size and n_blocks >= 1")
+    dev = _dev_index(block_tables)
+    positions, q_start, lengths, held_out, n_new = torch.empty(
+        n_rows + 3 * B + 1, dtype=torch.int32, device=device).split_with_sizes((n_rows, B, B, B, 1))
+    slots = torch.empty(n_rows, dtype=torch.int64, device=device)
+    _call(dev, "mz_paged_plan", block_tables.data_ptr(), max(width, 1), ctx_lens.data_ptr(),
+          q_lens.data_ptr(), _ptr(held), _ptr(new_ids), 0 if new_ids is None else new_ids.numel(),
+          B, n_rows, block_size, n_blocks, q_start.data_ptr(), positions.data_ptr(),
+          slots.data_ptr(), lengths.data_ptr(), held_out.data_ptr(), n_new.data_ptr())
+    return PagedPlan(q_start, positions, slots, lengths, held_out, n_new)
+
+
+# ---------------------------------------------------------------------------
+# Query / key norm, rotation and append
+# ---------------------------------------------------------------------------
+
+def _rope_args(q, k, positions, inv_freq, q_weight, k_weight, eps, weight_offset, interleaved,
+               freq_axes):
+    """Checks shared by the norm-and-rotation calls; the trailing arguments of
+    mz_qk_norm_rope from ``positions`` to ``norm``."""
+    T, Hq, D = q.shape
+    device = q.device
+    _as_i32(positions, device, "positions")
+    n_axes = 1 if positions.dim() == 1 else positions.shape[0]
+    if positions.dim() > 2 or positions.shape[-1] != T:
+        raise ValueError(f"positions must be int32 [{T}] or [axes, {T}]")
+    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or inv_freq.device != device or \
+            not inv_freq.is_contiguous():
+        raise ValueError(f"inv_freq must be a contiguous 1-D float32 tensor on {device}")
+    half = inv_freq.numel()
+    if freq_axes is not None:
+        _as_i32(freq_axes, device, "freq_axes")
+        if freq_axes.numel() != half:
+            raise ValueError("freq_axes must name one position axis per frequency")
+    elif n_axes > 1 and half:
+        raise ValueError("several position axes need freq_axes")
+    w = q_weight if q_weight is not None else k_weight
+    if w is not None and eps is None:
+        raise ValueError("norm weights need eps")
+    for x in (q_weight, k_weight):
+        if x is not None and (x.shape != (D,) or x.dtype != w.dtype or x.device != device
+                              or not x.is_contiguous()):
+            raise ValueError(f"norm weights must be contiguous [{D}] of one dtype on {device}")
+    return (positions.data_ptr(), T, n_axes, inv_freq.data_ptr(), _ptr(freq_axes), 2 * half,
+            1 if interleaved else 0, _ptr(q_weight), _ptr(k_weight),
+            0 if w is None else dtype_code(w.dtype), float(weight_offset),
+            0.0 if eps is None else float(eps), 0 if eps is None else 1)
+
+
+def _check_heads(t: torch.Tensor, name: str, like: torch.Tensor) -> None:
+    if t.dim() != 3 or t.shape[0] != like.shape[0] or t.shape[2] != like.shape[2] or \
+            t.stride(2) != 1 or t.dtype != like.dtype or t.device != like.device:
+        raise ValueError(f"{name} must be [{like.shape[0]}, heads, {like.shape[2]}] of "
+                         f"{like.dtype} on {like.device} with unit last stride")
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
+                 inv_freq: torch.Tensor, q_weight: torch.Tensor | None = None,
+                 k_weight: torch.Tensor | None = None, eps: float | None = None,
+                 weight_offset: float = 0.0, interleaved: bool = False,
+                 freq_axes: torch.Tensor | None = None, q_out: torch.Tensor | None = None,
+                 k_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """RMS norm of each head of q ``[T, Hq, D]`` and k ``[T, Hkv, D]`` and their
+    rotation by position, in one pass (mz_qk_norm_rope).
+
+    positions: int32 ``[T]``, or ``[axes, T]`` with ``freq_axes`` int32
+    ``[len(inv_freq)]`` naming the axis of every frequency (time, height and
+    width of image or video tokens, say).  The first ``2 * len(inv_freq)``
+    dimensions rotate by ``position * inv_freq[i]`` (float32), as pairs
+    ``(i, i + len(inv_freq))`` or, ``interleaved``, ``(2i, 2i + 1)``.  The norm
+    runs if ``eps`` is given, times ``weight + weight_offset`` where a weight
+    is.  ``q_out`` / ``k_out`` may be q / k themselves."""
+    if q.dim() != 3 or q.stride(2) != 1:
+        raise ValueError("q must be [T, heads, D] with unit last stride")
+    _check_heads(k, "k", q)
+    args = _rope_args(q, k, positions, inv_freq, q_weight, k_weight, eps, weight_offset,
+                      interleaved, freq_axes)
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if k_out is None:
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    _check_heads(q_out, "q_out", q)
+    _check_heads(k_out, "k_out", k)
+    if q_out.shape != q.shape or k_out.shape != k.shape:
+        raise ValueError("q_out and k_out must match q and k")
+    _call(_dev_index(q), "mz_qk_norm_rope", q_out.data_ptr(), q_out.stride(0), q_out.stride(1),
+          k_out.data_ptr(), k_out.stride(0), k_out.stride(1), q.data_ptr(), q.stride(0),
+          q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), None, 0, 0, None, None, None, 0, 0,
+          *args, q.shape[0], q.shape[1], k.shape[1], q.shape[2], dtype_code(q.dtype))
+    return q_out, k_out
+
+
+def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                        positions: torch.Tensor, inv_freq: torch.Tensor, k_pool: torch.Tensor,
+                        v_pool: torch.Tensor, slot_mapping: torch.Tensor,
+                        q_weight: torch.Tensor | None = None,
+                        k_weight: torch.Tensor | None = None, eps: float | None = None,
+                        weight_offset: float = 0.0, interleaved: bool = False,
+                        freq_axes: torch.Tensor | None = None,
+                        q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """``qk_norm_rope`` and ``kv_append`` in one pass: the queries go to the
+    returned tensor (or ``q_out``, which may be q), the keys and v ``[T, Hkv, D]``
+    to their slots of the pools.  slot_mapping: int64 ``[T]``, distinct; a
+    negative slot skips the write."""
+    n_blocks, H, bs, D = _check_pools(k_pool, v_pool)
+    if q.dim() != 3 or q.shape[2] != D or q.stride(2) != 1 or q.dtype != k_pool.dtype or \
+            q.device != k_pool.device:
+        raise ValueError(f"q must be [T, heads, {D}] of the pools' dtype and device with unit "
+                         "last stride")
+    _check_heads(k, "k", q)
+    _check_heads(v, "v", q)
+    if k.shape[1] != H or v.shape[1] != H:
+        raise ValueError(f"k and v must have the pools' {H} heads")
+    T = q.shape[0]
+    if slot_mapping.dtype != torch.int64 or slot_mapping.numel() != T or \
+            slot_mapping.device != q.device or not slot_mapping.is_contiguous():
+        raise ValueError("slot_mapping must be a contiguous int64 [T] on the pool device")
+    args = _rope_args(q, k, positions, inv_freq, q_weight, k_weight, eps, weight_offset,
+                      interleaved, freq_axes)
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _check_heads(q_out, "q_out", q)
+    if q_out.shape != q.shape:
+        raise ValueError("q_out must match q")
+    _call(_dev_index(q), "mz_qk_norm_rope", q_out.data_ptr(), q_out.stride(0), q_out.stride(1),
+          None, 0, 0, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0),
+          k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), k_pool.data_ptr(),
+          v_pool.data_ptr(), slot_mapping.data_ptr(), bs, n_blocks, *args, T, q.shape[1], H, D,
+          dtype_code(q.dtype))
+    return q_out
+
+
+# ---------------------------------------------------------------------------
 # Decode attention
 # ---------------------------------------------------------------------------
 
@@ -237,6 +422,33 @@ def decode_workspace(n_seqs: int, n_kv_heads: int, rows: int, head_dim: int, dev
     return _layout_workspace(_workspaces, key, int(size.value), device, shared)
 
 
+def _score_mod(n_heads: int, device: torch.device, softcap: float,
+               alibi_slopes: torch.Tensor | None, window: int, sink_tokens: int,
+               prefix_lens: torch.Tensor | None, first_keys: torch.Tensor | None, n_seqs: int,
+               n_first: int) -> "nat.ScoreMod | None":
+    """The checked mz_score_mod of an attention call; None where nothing of it
+    is in use (the sink tokens alone change nothing)."""
+    if softcap < 0 or not math.isfinite(softcap):
+        raise ValueError("softcap must be finite and not negative (0: none)")
+    if window < 0 or sink_tokens < 0:
+        raise ValueError("window and sink_tokens must not be negative")
+    if alibi_slopes is not None and (
+            alibi_slopes.dtype != torch.float32 or alibi_slopes.shape != (n_heads,) or
+            alibi_slopes.device != device or not alibi_slopes.is_contiguous()):
+        raise ValueError(f"alibi_slopes must be a contiguous float32 [{n_heads}] on {device}")
+    for t, name, n in ((prefix_lens, "prefix_lens", n_seqs), (first_keys, "first_keys", n_first)):
+        if t is not None:
+            _as_i32(t, device, name)
+            if t.numel() != n:
+                raise ValueError(f"{name} must hold {n} entries")
+    if not (softcap or window or alibi_slopes is not None or prefix_lens is not None
+            or first_keys is not None):
+        return None
+    big = (1 << 31) - 1
+    return nat.ScoreMod(softcap, min(window, big), min(sink_tokens, big), _ptr(alibi_slopes),
+                        _ptr(prefix_lens), _ptr(first_keys))
+
+
 def reset_workspaces() -> None:
     """Zero every cached workspace (needed after a call that reported an error)."""
     for ws in list(_workspaces.values()) + list(_qworkspaces.values()):
@@ -246,11 +458,24 @@ def reset_workspaces() -> None:
 def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
                  block_tables: torch.Tensor, ctx_lens: torch.Tensor, scale: float | None = None,
                  out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,
-                 num_warps: int = 0, workspace: torch.Tensor | None = None) -> torch.Tensor:
+                 num_warps: int = 0, workspace: torch.Tensor | None = None, causal: bool = False,
+                 softcap: float = 0.0, alibi_slopes: torch.Tensor | None = None, window: int = 0,
+                 sink_tokens: int = 0, prefix_lens: torch.Tensor | None = None,
+                 first_keys: torch.Tensor | None = None) -> torch.Tensor:
     """Fused GQA paged decode attention.
 
     q: ``[B, Hq, D]`` (one query token per sequence) or ``[B, n_q, Hq, D]``.
     Returns ``out`` with q's shape, dtype ``out_dtype`` (default q.dtype).
+
+    ``causal``: the n_q tokens are the sequence's last ones (drafted tokens,
+    say) and each sees the keys up to its own; without it all see every key.
+    Modified scores and masks (mz_score_mod; several tokens then need
+    ``causal``): ``softcap`` caps the scaled scores by ``softcap * tanh(x /
+    softcap)``; ``alibi_slopes`` float32 ``[Hq]`` subtracts ``slope * distance``;
+    a token sees the last ``window`` keys (0: all), not those before
+    ``first_keys[b]`` (its document's start), and in any case the first
+    ``sink_tokens`` and the first ``prefix_lens[b]``.  A token that sees no key
+    gets zeros; blocks that no token sees need no valid table entry.
     """
     n_blocks, Hkv, bs, D = _check_pools(k_pool, v_pool)
     if q.dtype != k_pool.dtype:
@@ -283,12 +508,25 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         o_sb, o_st, o_sh = out.stride(0), out.stride(1), out.stride(2)
     if scale is None:
         scale = D ** -0.5
+    mod = _score_mod(Hq, q.device, softcap, alibi_slopes, window, sink_tokens, prefix_lens,
+                     first_keys, B, B)
+    if mod is not None and nq > 1 and not causal:
+        raise ValueError("modified scores of several query tokens need causal=True")
+    if mod is None and causal and nq > 1:
+        mod = nat.ScoreMod()
     if B == 0:
         return out
     dev = _dev_index(q)
     rows = nq * (Hq // Hkv)
     if workspace is None:
         workspace = decode_workspace(B, Hkv, rows, D, dev, num_warps)
+    if mod is not None:
+        _call(dev, "mz_paged_decode_mod", out.data_ptr(), dtype_code(out_dtype), o_sb, o_st, o_sh,
+              q.data_ptr(), q_sb, q_st, q_sh, nq, k_pool.data_ptr(), v_pool.data_ptr(),
+              block_tables.data_ptr(), block_tables.shape[1], ctx_lens.data_ptr(), B, Hq, Hkv, D,
+              bs, n_blocks, float(scale), ctypes.byref(mod), dtype_code(q.dtype), num_warps,
+              workspace.data_ptr(), workspace.numel())
+        return out
     nat.call("mz_paged_decode", out.data_ptr(), dtype_code(out_dtype), o_sb, o_st, o_sh,
              q.data_ptr(), q_sb, q_st, q_sh, nq, k_pool.data_ptr(), v_pool.data_ptr(),
              block_tables.data_ptr(), block_tables.shape[1], ctx_lens.data_ptr(), B, Hq, Hkv,
@@ -303,8 +541,11 @@ def paged_append_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Ten
                         ctx_lens: torch.Tensor, scale: float | None = None,
                         out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,
                         num_warps: int = 0, workspace: torch.Tensor | None = None,
-                        overlap_previous: bool = False,
-                        batch_invariant: bool = False) -> torch.Tensor:
+                        overlap_previous: bool = False, batch_invariant: bool = False,
+                        softcap: float = 0.0, alibi_slopes: torch.Tensor | None = None,
+                        window: int = 0, sink_tokens: int = 0,
+                        prefix_lens: torch.Tensor | None = None,
+                        first_keys: torch.Tensor | None = None) -> torch.Tensor:
     """Fused decode step for one layer: write ``k_new/v_new [B, Hkv, D]`` at
     position ``ctx_lens[b] - 1`` of each sequence, then attend ``q [B, Hq, D]``
     over the first ``ctx_lens[b]`` tokens (one launch).  ``overlap_previous``:
@@ -312,7 +553,8 @@ def paged_append_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Ten
     (MZ_LAUNCH_OVERLAP_PREVIOUS) -- only when that kernel writes none of the
     pools, ``block_tables`` or ``ctx_lens``.  ``batch_invariant``: each
     sequence's output bytes are independent of the rest of the batch
-    (MZ_DECODE_BATCH_INVARIANT)."""
+    (MZ_DECODE_BATCH_INVARIANT).  Modified scores and masks as in
+    ``paged_decode``."""
     n_blocks, Hkv, bs, D = _check_pools(k_pool, v_pool)
     if q.dim() != 3 or q.shape[2] != D or q.stride(-1) != 1 or q.dtype != k_pool.dtype:
         raise ValueError(f"q must be [B, Hq, {D}] of the pool dtype with unit last stride")
@@ -332,6 +574,8 @@ def paged_append_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Ten
         raise ValueError("out must match q's shape with unit last stride")
     if scale is None:
         scale = D ** -0.5
+    mod = _score_mod(Hq, q.device, softcap, alibi_slopes, window, sink_tokens, prefix_lens,
+                     first_keys, B, B)
     if B == 0:
         return out
     dev = _dev_index(q)
@@ -339,6 +583,17 @@ def paged_append_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Ten
         workspace = decode_workspace(B, Hkv, Hq // Hkv, D, dev, num_warps,
                                      batch_invariant=batch_invariant,
                                      max_blocks=block_tables.shape[1], block_size=bs)
+    if mod is not None:
+        _call(dev, "mz_paged_append_decode_mod", out.data_ptr(), dtype_code(out_dtype),
+              out.stride(0), out.stride(1), q.data_ptr(), q.stride(0), q.stride(1),
+              k_pool.data_ptr(), v_pool.data_ptr(), k_new.data_ptr(), v_new.data_ptr(),
+              k_new.stride(0), k_new.stride(1), block_tables.data_ptr(), block_tables.shape[1],
+              ctx_lens.data_ptr(), B, Hq, Hkv, D, bs, n_blocks, float(scale), ctypes.byref(mod),
+              dtype_code(q.dtype), num_warps,
+              (nat.MZ_LAUNCH_OVERLAP_PREVIOUS if overlap_previous else 0)
+              | (nat.MZ_DECODE_BATCH_INVARIANT if batch_invariant else 0),
+              workspace.data_ptr(), workspace.numel())
+        return out
     nat.call("mz_paged_append_decode_ex", out.data_ptr(), dtype_code(out_dtype), out.stride(0),
              out.stride(1), q.data_ptr(), q.stride(0), q.stride(1), k_pool.data_ptr(),
              v_pool.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), k_new.stride(0),
@@ -355,12 +610,16 @@ def paged_append_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Ten
 def paged_prefill(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
                   block_tables: torch.Tensor, q_start: torch.Tensor, q_len: torch.Tensor,
                   ctx_lens: torch.Tensor, max_q_len: int, scale: float | None = None,
-                  out: torch.Tensor | None = None,
-                  out_dtype: torch.dtype | None = None) -> torch.Tensor:
+                  out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,
+                  softcap: float = 0.0, alibi_slopes: torch.Tensor | None = None,
+                  window: int = 0, sink_tokens: int = 0,
+                  prefix_lens: torch.Tensor | None = None,
+                  first_keys: torch.Tensor | None = None) -> torch.Tensor:
     """Chunked prefill attention (mz_paged_prefill): ``q [T, Hq, D]`` holds
     sequence b's ``q_len[b]`` query tokens at rows ``q_start[b]...``; they sit
     at the last ``q_len[b]`` of the sequence's ``ctx_lens[b]`` positions (their
-    K/V already appended) and attend causally."""
+    K/V already appended) and attend causally.  Modified scores and masks as in
+    ``paged_decode``, with ``first_keys`` int32 ``[T]``, one per row of q."""
     n_blocks, Hkv, bs, D = _check_pools(k_pool, v_pool)
     if q.dim() != 3 or q.shape[2] != D or q.stride(-1) != 1 or q.dtype != k_pool.dtype:
         raise ValueError(f"q must be [T, Hq, {D}] of the pool dtype with unit last stride")
@@ -378,9 +637,18 @@ def paged_prefill(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         raise ValueError("out must match q's shape with unit last stride")
     if scale is None:
         scale = D ** -0.5
+    mod = _score_mod(Hq, q.device, softcap, alibi_slopes, window, sink_tokens, prefix_lens,
+                     first_keys, B, T)
     if B == 0 or T == 0 or max_q_len == 0:
         return out
     dev = _dev_index(q)
+    if mod is not None:
+        _call(dev, "mz_paged_prefill_mod", out.data_ptr(), dtype_code(out_dtype), out.stride(0),
+              out.stride(1), q.data_ptr(), q.stride(0), q.stride(1), T, q_start.data_ptr(),
+              q_len.data_ptr(), int(max_q_len), k_pool.data_ptr(), v_pool.data_ptr(),
+              block_tables.data_ptr(), block_tables.shape[1], ctx_lens.data_ptr(), B, Hq, Hkv, D,
+              bs, n_blocks, float(scale), ctypes.byref(mod), dtype_code(q.dtype))
+        return out
     nat.call("mz_paged_prefill", out.data_ptr(), dtype_code(out_dtype), out.stride(0),
              out.stride(1), q.data_ptr(), q.stride(0), q.stride(1), T, q_start.data_ptr(),
              q_len.data_ptr(), int(max_q_len), k_pool.data_ptr(), v_pool.data_ptr(),

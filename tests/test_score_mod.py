@@ -1,0 +1,450 @@
+"""Attention over the paged cache with capped scores, a bias by distance, a
+window with sink tokens, prefix and document masks: decode (single tokens and
+drafted runs), fused append and decode, and chunked prefill, against float64.
+
+Tolerance, per element, with u = eps/2 of the output type and ``spread`` the
+softmax-weighted sum of |v|:  u |ref| + 2^-10 spread (+ fp16's smallest step).
+The kernels hold P in fp16 (relative 2^-11) or in two bf16 parts (2^-17), which
+moves the numerator by that share of ``spread``; the other 2^-11 allows the
+scores an absolute error of 2^-12, twice (numerator and row sum): fp32 dot
+products of up to 128 terms of size 4 sum to errors below 128 * 2^-24 * 16, the
+cap's tanh is within 1e-6 of 50, the bias within 2^-24 of its size where the
+key still counts (below 100), the exponential within 2^-22."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from mlxz_b200 import _native, ops
+from mlxz_b200._native import DeviceError
+from oracle import rng
+from oracle import score_mod as osm
+from tests.gpu_util import TORCH, random_paged_case, to_bits, to_dev
+
+gpu = pytest.mark.gpu
+
+
+def _check(out, want, what=""):
+    ref, spread = want
+    u = 0.0 if out.dtype == torch.float32 else torch.finfo(out.dtype).eps / 2
+    tiny = 2.0 ** -25 if out.dtype == torch.float16 else 0.0
+    o = out.detach().float().cpu().numpy().astype(np.float64).reshape(ref.shape)
+    tol = u * np.abs(ref) + 2.0 ** -10 * spread + tiny
+    bad = ~(np.abs(o - ref) <= tol)
+    assert not bad.any(), (what, int(bad.sum()), float(np.abs(o - ref)[bad].max()))
+
+
+MODS = {
+    "cap": dict(softcap=20.0),
+    "slopes": dict(slopes=True),
+    "window": dict(window=37),
+    "window1": dict(window=1),
+    "window_sink": dict(window=64, sink=4),
+    "window_sinks": dict(window=16, sink=33),
+    "far_sink": dict(window=5, sink=5000),
+    "docs": dict(docs=50),
+    "prefix": dict(prefix=29, window=20),
+    "all": dict(softcap=50.0, slopes=True, window=100, sink=3, docs=130, prefix=10),
+}
+
+
+def _mod_args(mod, Hq, ctx, q_len, per_row, cuda):
+    """(keyword arguments of ops, of the oracle) for a mod of MODS."""
+    kw, ow = {}, {}
+    if mod.get("softcap"):
+        kw["softcap"] = ow["softcap"] = mod["softcap"]
+    if mod.get("slopes"):
+        s = (2.0 ** (-8.0 * (np.arange(Hq) + 1) / Hq)).astype(np.float32)
+        kw["alibi_slopes"], ow["slopes"] = torch.from_numpy(s).to(cuda), s
+    if mod.get("window"):
+        kw["window"] = ow["window"] = mod["window"]
+        kw["sink_tokens"] = ow["sink"] = mod.get("sink", 0)
+    if mod.get("prefix"):
+        # ragged: 0, the full length and beyond among them
+        p = np.array([(mod["prefix"] * (b % 4)) for b in range(len(ctx))], dtype=np.int32)
+        kw["prefix_lens"], ow["prefix"] = torch.from_numpy(p).to(cuda), p
+    if mod.get("docs"):
+        d = mod["docs"]
+        if per_row:
+            f = np.concatenate([np.arange(c - n, c) // d * d for c, n in zip(ctx, q_len)] or
+                               [np.zeros(0)]).astype(np.int32)
+            kw["first_keys"], ow["first"] = torch.from_numpy(f).to(cuda), f
+        else:
+            f = np.array([max(0, c - n) // d * d for c, n in zip(ctx, q_len)], dtype=np.int32)
+            kw["first_keys"] = torch.from_numpy(f).to(cuda)
+            ow["first"] = np.repeat(f, q_len)
+    return kw, ow
+
+
+def _dev(case, dtype, cuda):
+    return (to_dev(case["kp"], dtype, cuda), to_dev(case["vp"], dtype, cuda),
+            torch.from_numpy(case["tables"]).to(cuda), torch.from_numpy(case["ctx"]).to(cuda))
+
+
+# --- decode ---------------------------------------------------------------------------
+
+CTX = [300, 1, 15, 16, 17, 63, 64, 65, 0, 1000, 37, 129]
+
+
+@gpu
+@pytest.mark.parametrize("mod", MODS)
+@pytest.mark.parametrize("dtype,D,G,bs,nq", [("bf16", 128, 4, 16, 1), ("f16", 64, 4, 32, 3),
+                                             ("bf16", 64, 1, 48, 16), ("f16", 128, 16, 16, 1),
+                                             ("bf16", 128, 2, 64, 5)])
+def test_decode_vs_oracle(cuda, mod, dtype, D, G, bs, nq):
+    Hkv, B = 2, len(CTX)
+    case = random_paged_case(11 + D + nq, B, Hkv, D, bs, CTX, dtype, nq=nq, G=G)
+    kp, vp, tables, ctx = _dev(case, dtype, cuda)
+    q = to_dev(case["q"], dtype, cuda)
+    q_len = np.full(B, nq)
+    kw, ow = _mod_args(MODS[mod], Hkv * G, CTX, q_len, False, cuda)
+    out = ops.paged_decode(q, kp, vp, tables, ctx, causal=True, out_dtype=torch.float32, **kw)
+    torch.cuda.synchronize()
+    ops.check_device_errors(0)
+    rows = case["q"].reshape(B * nq, Hkv * G, D)
+    _check(out, osm.paged(rows, case["kp"], case["vp"], case["tables"], np.arange(B) * nq, q_len,
+                          case["ctx"], dtype, **ow), mod)
+
+
+@gpu
+@pytest.mark.parametrize("num_warps", [0, 4, 8, 64])
+@pytest.mark.parametrize("mod", ["window_sink", "all", "cap"])
+def test_decode_split_over_warps(cuda, num_warps, mod):
+    """Long contexts cut into pieces: some rows see nothing of some pieces."""
+    dtype, D, G, nq, ctx = "bf16", 128, 4, 4, [5000, 3, 2047, 700]
+    case = random_paged_case(3, 4, 2, D, 16, ctx, dtype, nq=nq, G=G)
+    kp, vp, tables, c = _dev(case, dtype, cuda)
+    q = to_dev(case["q"], dtype, cuda)
+    q_len = np.full(4, nq)
+    m = dict(MODS[mod], window=2000) if mod == "all" else MODS[mod]
+    kw, ow = _mod_args(m, 8, ctx, q_len, False, cuda)
+    out = ops.paged_decode(q, kp, vp, tables, c, causal=True, num_warps=num_warps, **kw)
+    torch.cuda.synchronize()
+    ops.check_device_errors(0)
+    _check(out, osm.paged(case["q"].reshape(16, 8, D), case["kp"], case["vp"], case["tables"],
+                          np.arange(4) * nq, q_len, case["ctx"], dtype, **ow), mod)
+
+
+@gpu
+def test_causal_without_mods_is_a_drafted_run(cuda):
+    """Row i of a drafted run is the plain decode over its own prefix."""
+    dtype, D, G, nq = "bf16", 64, 4, 4
+    ctx = [200, 33, 4]
+    case = random_paged_case(8, 3, 2, D, 16, ctx, dtype, nq=nq, G=G)
+    kp, vp, tables, c = _dev(case, dtype, cuda)
+    q = to_dev(case["q"], dtype, cuda)
+    out = ops.paged_decode(q, kp, vp, tables, c, causal=True)
+    _check(out, osm.paged(case["q"].reshape(12, 8, D), case["kp"], case["vp"], case["tables"],
+                          np.arange(3) * nq, np.full(3, nq), case["ctx"], dtype))
+    one = ops.paged_decode(q[:, -1], kp, vp, tables, c)
+    assert torch.equal(ops.paged_decode(q[:, -1], kp, vp, tables, c, causal=True), one)
+
+
+@gpu
+@pytest.mark.parametrize("nq", [1, 3])
+def test_rows_that_see_nothing_are_zero(cuda, nq):
+    """Documents that start behind the token; more drafted tokens than context."""
+    dtype, D, ctx = "f16", 128, [40, 2, 100, 0]
+    case = random_paged_case(5, 4, 2, D, 16, ctx, dtype, nq=nq, G=4)
+    kp, vp, tables, c = _dev(case, dtype, cuda)
+    first = torch.tensor([40, 0, 1 << 30, 0], dtype=torch.int32, device=cuda)
+    q = to_dev(case["q"], dtype, cuda)
+    out = torch.full_like(q, 7.0)
+    ops.paged_decode(q, kp, vp, tables, c, causal=True, first_keys=first, out=out)
+    torch.cuda.synchronize()
+    ops.check_device_errors(0)
+    assert not out[0].any() and not out[2].any() and not out[3].any()
+    assert not out[1, :max(0, nq - 2)].any() and out[1, -1].any()
+
+
+@gpu
+@pytest.mark.parametrize("fill", [float("nan"), float("inf"), 6e4])
+def test_decode_hidden_blocks_may_be_anything(cuda, fill):
+    """What the window leaves out may be NaN, infinite or gone: blocks behind it
+    lose their table entries, the rest of a partly seen tile holds ``fill``."""
+    dtype, D, G, ctx, window, sink = "f16", 64, 4, [500, 130, 77], 70, 5
+    case = random_paged_case(6, 3, 2, D, 16, ctx, dtype, G=G)
+    kp, vp, tables, c = _dev(case, dtype, cuda)
+    q = to_dev(case["q"][:, 0], dtype, cuda)
+    want = ops.paged_decode(q, kp, vp, tables, c, window=window, sink_tokens=sink)
+    for b, n in enumerate(ctx):
+        for t in range(sink, n - window):
+            blk = int(tables[b, t // 16])
+            kp[blk, :, t % 16] = fill
+            vp[blk, :, t % 16] = fill
+        for j in range(1, (n - window) // 16):
+            tables[b, j] = -1 if j % 2 else 1 << 30
+    got = ops.paged_decode(q, kp, vp, tables, c, window=window, sink_tokens=sink)
+    torch.cuda.synchronize()
+    ops.check_device_errors(0)
+    assert torch.equal(got, want)
+
+
+@gpu
+@pytest.mark.parametrize("batch_invariant", [False, True])
+@pytest.mark.parametrize("mod", ["cap", "window_sink", "docs", "all"])
+def test_append_decode_vs_oracle(cuda, batch_invariant, mod):
+    """The new token is written to its slot and attended in the same launch."""
+    dtype, D, G, Hkv = "bf16", 128, 4, 2
+    ctx = [300, 1, 16, 17, 2000, 129]
+    B = len(ctx)
+    case = random_paged_case(21, B, Hkv, D, 16, ctx, dtype, G=G)
+    kp, vp, tables, c = _dev(case, dtype, cuda)
+    q = to_dev(case["q"][:, 0], dtype, cuda)
+    kn, vn = (rng.normal(22, (B, Hkv, D), dtype, stream=s) for s in (1, 2))
+    kw, ow = _mod_args(MODS[mod], Hkv * G, ctx, np.ones(B, dtype=int), False, cuda)
+    out = ops.paged_append_decode(q, kp, vp, to_dev(kn, dtype, cuda), to_dev(vn, dtype, cuda),
+                                  tables, c, batch_invariant=batch_invariant, **kw)
+    torch.cuda.synchronize()
+    ops.check_device_errors(0)
+    for b, n in enumerate(ctx):
+        blk, at = case["tables"][b, (n - 1) // 16], (n - 1) % 16
+        case["kp"][blk, :, at], case["vp"][blk, :, at] = kn[b], vn[b]
+    assert np.array_equal(to_bits(kp), case["kp"]) and np.array_equal(to_bits(vp), case["vp"])
+    _check(out, osm.paged(case["q"][:, 0], case["kp"], case["vp"], case["tables"], np.arange(B),
+                          np.ones(B, dtype=int), case["ctx"], dtype, **ow), mod)
+
+
+@gpu
+def test_batch_invariant_bytes_with_a_window(cuda):
+    """A sequence's bytes do not depend on the batch around it."""
+    dtype, D, G, Hkv, ctx = "bf16", 64, 4, 2, [3000, 40, 900]
+    case = random_paged_case(23, 3, Hkv, D, 16, ctx, dtype, G=G)
+    kp, vp, tables, c = _dev(case, dtype, cuda)
+    q = to_dev(case["q"][:, 0], dtype, cuda)
+    kn = to_dev(rng.normal(24, (3, Hkv, D), dtype), dtype, cuda)
+    kw = dict(window=1500, sink_tokens=4, softcap=30.0, batch_invariant=True)
+    out = ops.paged_append_decode(q, kp, vp, kn, kn, tables, c, **kw)
+    for b in range(3):
+        s = slice(b, b + 1)
+        one = ops.paged_append_decode(q[s], kp, vp, kn[s], kn[s], tables[s].contiguous(), c[s], **kw)
+        assert torch.equal(one[0], out[b])
+
+
+@gpu
+def test_decode_graph_and_two_streams(cuda):
+    """Captured launches with their own workspaces on two streams at once, and
+    lengths that change between replays."""
+    dtype, D, G, ctx = "bf16", 128, 4, [900, 70]
+    case = random_paged_case(31, 2, 2, D, 16, [1000, 90], dtype, G=G)
+    kp, vp, tables, _ = _dev(case, dtype, cuda)
+    c = torch.tensor(ctx, dtype=torch.int32, device=cuda)
+    q = to_dev(case["q"][:, 0], dtype, cuda)
+    kw = dict(window=128, sink_tokens=4, softcap=30.0)
+    graphs, outs, streams = [], [], []
+    for _ in range(2):
+        ws = ops.decode_workspace(2, 2, G, D, 0, shared=False)
+        s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            ops.paged_decode(q, kp, vp, tables, c, workspace=ws, **kw)
+            with torch.cuda.graph(g, stream=s):
+                outs.append(ops.paged_decode(q, kp, vp, tables, c, workspace=ws, **kw))
+        graphs.append((g, ws))
+        streams.append(s)
+    torch.cuda.synchronize()
+    for lens in ([900, 70], [1000, 90], [40, 1]):
+        c.copy_(torch.tensor(lens, dtype=torch.int32))
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for (g, _), s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        want = osm.paged(case["q"][:, 0], case["kp"], case["vp"], case["tables"], np.arange(2),
+                         np.ones(2, dtype=int), np.array(lens), dtype, softcap=30.0, window=128,
+                         sink=4)
+        for o in outs:
+            _check(o, want, lens)
+    ops.check_device_errors(0)
+
+
+# --- prefill --------------------------------------------------------------------------
+
+def _prefill_case(seed, ctx, qlen, dtype, D, G, bs, Hkv):
+    case = random_paged_case(seed, len(ctx), Hkv, D, bs, ctx, dtype, G=G)
+    T = sum(qlen)
+    case["qp"] = rng.normal(seed, (max(T, 1), Hkv * G, D), dtype, stream=9)[:T]
+    case["q_start"] = np.cumsum([0] + qlen[:-1]).astype(np.int32)
+    case["q_len"] = np.array(qlen, dtype=np.int32)
+    return case
+
+
+def _prefill(case, dtype, cuda, kw, out_dtype=None, out=None, pools=None):
+    kp, vp, tables, ctx = pools or _dev(case, dtype, cuda)
+    i = {k: torch.from_numpy(case[k]).to(cuda) for k in ("q_start", "q_len")}
+    res = ops.paged_prefill(to_dev(case["qp"], dtype, cuda), kp, vp, tables, i["q_start"],
+                            i["q_len"], ctx, int(case["q_len"].max()), out_dtype=out_dtype,
+                            out=out, **kw)
+    torch.cuda.synchronize()
+    ops.check_device_errors(0)
+    return res
+
+
+PREFILL = [
+    # dtype, D, G, bs, ctx (chunk included), q_len
+    ("bf16", 128, 8, 16, [100, 300, 17, 64, 513], [100, 37, 1, 0, 200]),
+    ("f16", 64, 1, 16, [1000, 129], [513, 129]),
+    ("bf16", 64, 16, 32, [77, 40, 300], [30, 40, 299]),
+    ("f16", 128, 4, 64, [2000, 5], [200, 5]),
+    ("bf16", 128, 2, 48, [16, 33, 1, 385], [16, 33, 1, 385]),
+]
+
+
+@gpu
+@pytest.mark.parametrize("mod", MODS)
+@pytest.mark.parametrize("dtype,D,G,bs,ctx,qlen", PREFILL)
+def test_prefill_vs_oracle(cuda, mod, dtype, D, G, bs, ctx, qlen):
+    Hkv = 2
+    case = _prefill_case(40 + D + G, ctx, qlen, dtype, D, G, bs, Hkv)
+    kw, ow = _mod_args(MODS[mod], Hkv * G, ctx, qlen, True, cuda)
+    out = _prefill(case, dtype, cuda, kw, torch.float32)
+    _check(out, osm.paged(case["qp"], case["kp"], case["vp"], case["tables"], case["q_start"],
+                          case["q_len"], case["ctx"], dtype, **ow), mod)
+
+
+@gpu
+@pytest.mark.parametrize("window,sink", [(128, 0), (129, 4), (500, 128), (1000, 200), (4000, 4)])
+def test_prefill_long_window(cuda, window, sink):
+    """Windows that leave out whole key tiles, at and off their borders."""
+    case = _prefill_case(50, [3000, 900], [260, 130], "bf16", 128, 4, 16, 1)
+    out = _prefill(case, "bf16", cuda, dict(window=window, sink_tokens=sink))
+    _check(out, osm.paged(case["qp"], case["kp"], case["vp"], case["tables"], case["q_start"],
+                          case["q_len"], case["ctx"], "bf16", window=window, sink=sink))
+
+
+@gpu
+def test_prefill_prefix_ahead_of_the_chunk(cuda):
+    """A first chunk inside its prefix sees keys that lie ahead of it, several
+    key tiles on."""
+    ctx, qlen, pre = [700, 700, 300], [40, 700, 100], np.array([650, 650, 900], dtype=np.int32)
+    case = _prefill_case(51, ctx, qlen, "bf16", 64, 2, 16, 2)
+    for kw in ({}, dict(window=30), dict(softcap=20.0)):
+        out = _prefill(case, "bf16", cuda, dict(kw, prefix_lens=torch.from_numpy(pre).to(cuda)))
+        _check(out, osm.paged(case["qp"], case["kp"], case["vp"], case["tables"],
+                              case["q_start"], case["q_len"], case["ctx"], "bf16", prefix=pre,
+                              **kw), kw)
+
+
+@gpu
+def test_prefill_empty_rows_and_rows_of_no_sequence(cuda):
+    """Rows that see nothing are zero; rows behind the last sequence stay."""
+    case = _prefill_case(52, [300, 140], [200, 130], "f16", 128, 4, 16, 2)
+    T = 330
+    first = np.zeros(T + 9, dtype=np.int32)
+    first[50:180] = 1 << 30      # more than a whole query block of empty rows
+    first[200:330] = np.arange(130) + 10 - 3
+    case["qp"] = rng.normal(52, (T + 9, 8, 128), "f16", stream=9)
+    out = torch.full((T + 9, 8, 128), 7.0, dtype=torch.float16, device=cuda)
+    _prefill(case, "f16", cuda, dict(first_keys=torch.from_numpy(first).to(cuda)), out=out)
+    assert not out[50:180].any() and (out[T:] == 7).all()
+    want = osm.paged(case["qp"], case["kp"], case["vp"], case["tables"], case["q_start"],
+                     case["q_len"], case["ctx"], "f16", first=first)
+    _check(out[:T], (want[0][:T], want[1][:T]))
+
+
+@gpu
+@pytest.mark.parametrize("fill", [float("nan"), float("inf")])
+def test_prefill_hidden_blocks_may_be_anything(cuda, fill):
+    ctx, qlen, window, sink = [900, 400], [100, 40], 150, 20
+    case = _prefill_case(53, ctx, qlen, "bf16", 128, 4, 16, 2)
+    kw = dict(window=window, sink_tokens=sink)
+    want = _prefill(case, "bf16", cuda, kw)
+    kp, vp, tables, c = _dev(case, "bf16", cuda)
+    for b, (n, m) in enumerate(zip(ctx, qlen)):
+        lo = n - m - window + 1  # the first row's lowest key
+        for t in range(sink, lo):
+            blk = int(tables[b, t // 16])
+            kp[blk, :, t % 16] = fill
+            vp[blk, :, t % 16] = fill
+        for j in range(-(-sink // 16), lo // 16):
+            tables[b, j] = -1
+    got = _prefill(case, "bf16", cuda, kw, pools=(kp, vp, tables, c))
+    # G = 4: a query block is 32 tokens, the later ones' hidden keys include seen ones
+    assert torch.equal(got, want)
+
+
+@gpu
+def test_prefill_last_row_equals_decode(cuda):
+    case = _prefill_case(54, [700, 250], [64, 9], "f16", 128, 8, 16, 1)
+    kw = dict(softcap=30.0, window=200, sink_tokens=4)
+    out = _prefill(case, "f16", cuda, kw, torch.float32)
+    kp, vp, tables, ctx = _dev(case, "f16", cuda)
+    last = case["q_start"] + case["q_len"] - 1
+    dec = ops.paged_decode(to_dev(case["qp"][last], "f16", cuda), kp, vp, tables, ctx,
+                           out_dtype=torch.float32, **kw)
+    want = osm.paged(case["qp"], case["kp"], case["vp"], case["tables"], case["q_start"],
+                     case["q_len"], case["ctx"], "f16", softcap=30.0, window=200, sink=4)
+    rows = (want[0][last], want[1][last])
+    _check(out[torch.from_numpy(last).long()], rows)
+    _check(dec, rows)
+
+
+# --- refusals -------------------------------------------------------------------------
+
+def _host(B=2, Hq=8, Hkv=2, D=64, nq=None):
+    q = torch.zeros(B, Hq, D, dtype=torch.bfloat16) if nq is None else \
+        torch.zeros(B, nq, Hq, D, dtype=torch.bfloat16)
+    pool = torch.zeros(4, Hkv, 16, D, dtype=torch.bfloat16)
+    return q, pool, pool, torch.zeros(B, 2, dtype=torch.int32), torch.ones(B, dtype=torch.int32)
+
+
+BAD = [(dict(softcap=-1.0), "softcap"), (dict(softcap=float("nan")), "softcap"),
+       (dict(window=-1), "window"), (dict(window=3, sink_tokens=-1), "sink"),
+       (dict(alibi_slopes=torch.zeros(8, dtype=torch.float64)), "alibi_slopes"),
+       (dict(alibi_slopes=torch.zeros(2)), "alibi_slopes"),
+       (dict(prefix_lens=torch.zeros(3, dtype=torch.int32)), "prefix_lens"),
+       (dict(prefix_lens=torch.zeros(2, dtype=torch.int64)), "prefix_lens"),
+       (dict(first_keys=torch.zeros(5, dtype=torch.int32)), "first_keys")]
+
+
+@pytest.mark.parametrize("kw,text", BAD)
+def test_refusals_on_the_host(kw, text):
+    q, kp, vp, tables, ctx = _host()
+    with pytest.raises(ValueError, match=text):
+        ops.paged_decode(q, kp, vp, tables, ctx, **kw)
+    k = torch.zeros(2, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match=text):
+        ops.paged_append_decode(q, kp, vp, k, k, tables, ctx, **kw)
+    with pytest.raises(ValueError, match=text):
+        ops.paged_prefill(q, kp, vp, tables, ctx, ctx, ctx, 1, **kw)
+
+
+def test_several_tokens_need_causal():
+    q, kp, vp, tables, ctx = _host(nq=3)
+    with pytest.raises(ValueError, match="causal"):
+        ops.paged_decode(q, kp, vp, tables, ctx, window=4)
+
+
+def test_c_abi_argument_errors():
+    lib = _native.lib()
+    p = ctypes.c_void_p(64)  # never read: every call below is refused first
+
+    def prefill(mod, D=64):
+        return lib.mz_paged_prefill_mod(p, 1, 512, 64, p, 512, 64, 4, p, p, 4, p, p, p, 2, p, 1, 8,
+                                        2, D, 16, 4, 0.125, mod, 1, None, None)
+
+    def append(mod):
+        return lib.mz_paged_append_decode_mod(p, 1, 512, 64, p, 512, 64, p, p, p, p, 128, 64, p, 2,
+                                              p, 1, 8, 2, 64, 16, 4, 0.125, mod, 1, 0, 0, p, 0,
+                                              None, None)
+
+    inv, ali = _native.MZ_ERR_INVALID_ARG, _native.MZ_ERR_ALIGNMENT
+    for fields, rc in ((dict(softcap=-2.0), inv), (dict(softcap=float("inf")), inv),
+                       (dict(window=-1), inv), (dict(sink_tokens=-3), inv),
+                       (dict(alibi_slopes=66), ali), (dict(prefix_lens=65), ali),
+                       (dict(first_keys=67), ali)):
+        assert append(ctypes.byref(_native.ScoreMod(**fields))) == rc, fields
+    assert prefill(None) == inv and append(None) == inv
+    ok = ctypes.byref(_native.ScoreMod(softcap=3.0))
+    assert prefill(ok, D=96) == _native.MZ_ERR_UNSUPPORTED
+
+
+def test_oracle_masks():
+    """The visibility rule on a case small enough to read."""
+    v = osm.visible(np.array([5]), 8, window=2, sink=1)[0]
+    assert v.tolist() == [True, False, False, False, True, True, False, False]
+    v = osm.visible(np.array([1, 5]), 8, window=2, prefix=3, first=np.array([0, 5]))
+    assert v[0].tolist() == [True] * 3 + [False] * 5
+    assert v[1].tolist() == [True] * 3 + [False] * 2 + [True] + [False] * 2
