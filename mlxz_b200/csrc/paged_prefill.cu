@@ -8,79 +8,11 @@
 // Tensor-core form (tcgen05 + TMEM), see the kernel's own comment below.
 // Shapes: head_dim 64 or 128, n_heads / n_kv_heads dividing 128, block_size a
 // multiple of 16, scale > 0 (the row max is taken on the raw scores).
-#include <climits>
-
-#include "decode_common.cuh"
+#include "prefill_common.cuh"
 #include "tcgen05.cuh"
 
 namespace mz {
 namespace prefill {
-
-using decode::kTileTok;
-using decode::kTimeoutNs;
-
-struct PParams {
-  void *out;
-  int64_t o_st, o_sh;  // out element (row t of the call, head hq, dim d)
-  int out_f32;
-  const void *q;
-  int64_t q_st, q_sh;
-  int n_rows;              // rows of q / out
-  const int32_t *q_start;  // [B] first row of sequence b in q / out
-  const int32_t *q_len;    // [B] query tokens of sequence b
-  const int32_t *ctx;      // [B] tokens in the pools, the chunk included
-  const int32_t *tables;
-  int max_blocks;
-  int Hkv, G, bs;
-  int64_t n_blocks;
-  float scale_log2;
-  int sub_log2;      // rows per bulk copy box: gcd(block_size, 128) = 1 << sub_log2
-  int32_t *err;
-  int n_seqs, qblocks;  // persistent form: sequences, query blocks per sequence
-  ScoreMod mod{};       // modified scores and masks
-};
-
-// 4-D bulk tensor copy (no multicast): box {64, 8, D / 64, rows / 8} of the
-// grouped map at row group `grp`.
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void *tmap, int grp, uint32_t bar,
-                                            uint64_t policy) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
-      " [%0], [%1, {%2, %2, %2, %3}], [%4], %5;" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(0), "r"(grp), "r"(bar), "l"(policy)
-      : "memory");
-}
-
-// Pool [rows][D] viewed as 4-D: (64 columns, 8 rows, D / 64 chunks, rows / 8
-// groups) with strides (row D*2 B, chunk 128 B, group 8*D*2 B), box {64, 8,
-// D / 64, box_rows / 8}, 128-byte swizzle: one copy brings box_rows whole rows
-// in the grouped layout the MMA descriptors read.
-inline int make_group_map(CUtensorMap *m, const void *base, int64_t rows, int D,
-                          CUtensorMapDataType type, int box_rows) {
-  auto fn = decode::encode_fn();
-  if (!fn) return fail(MZ_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
-  cuuint64_t dims[4] = {64, 8, static_cast<cuuint64_t>(D / 64), static_cast<cuuint64_t>(rows / 8)};
-  cuuint64_t strides[3] = {static_cast<cuuint64_t>(D) * 2, 128, static_cast<cuuint64_t>(D) * 16};
-  cuuint32_t box[4] = {64, 8, static_cast<cuuint32_t>(D / 64),
-                       static_cast<cuuint32_t>(box_rows / 8)};
-  cuuint32_t es[4] = {1, 1, 1, 1};
-  CUresult r = fn(m, type, 4, const_cast<void *>(base), dims, strides, box, es,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  if (r != CUDA_SUCCESS) return fail(MZ_ERR_CUDA, "cuTensorMapEncodeTiled (grouped) failed (%d)", (int)r);
-  return MZ_OK;
-}
-
-// max(a, b, c) in one instruction (three-input max.f32 of sm_100)
-__device__ __forceinline__ float fmax3f(float a, float b, float c) {
-  float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
-  return r;
-}
-
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
 
 // ---------------------------------------------------------------------------
 // One CTA per (128 query rows, KV head, sequence): row m is
@@ -108,7 +40,6 @@ __device__ __forceinline__ void mbar_arrive(uint32_t bar) {
 // abort flag, every role leaves its loop, the issuing threads wait (bounded)
 // for their copies / MMAs in flight, and warp 9 frees the TMEM.
 namespace tcp {
-constexpr int kM = 128;
 constexpr int kN = 128;
 constexpr int kKRing = 3;
 constexpr int kVRing = 2;
@@ -592,14 +523,7 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
 // PV of an item, which starts O afresh, waits until the softmax warps have
 // read the previous item's O (kBarOFree).  Everything else is the one-block
 // kernel above.
-//
-// MODE: 0 the causal mask alone; modified scores and masks (score_mod.cuh) from
-// 1 on: 1 masks, 2 masks and the bias by distance, 3 these and capped scores.
-// An item then reads the key tiles up to the last that every row sees (the
-// prefix and sink tokens) and those from its first row's lowest key on, local
-// tile t being tile t or t + skip of the sequence.  From 2 on the scores are
-// brought to their final form (log2 units) before the maximum is taken.
-template <int D, bool BF16, int MODE>
+template <int D, bool BF16>
 __global__ void __launch_bounds__(tcp::kThreads, 1)
     paged_prefill_ps_kernel(const __grid_constant__ CUtensorMap tmK,
                             const __grid_constant__ CUtensorMap tmV, const PParams p) {
@@ -615,9 +539,6 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
   struct Item {
     int b, h, q0, n, start, q_hi, kv_len, ntiles;
     bool ok;
-    // MODE > 0: keys [0, prefix) and [0, head) as in MaskSpan, the rows' lowest
-    // key lo, the head's tiles and the tiles left out behind them
-    int prefix, head, lo, head_tiles, skip;
   };
   auto item_at = [&](int e) {
     Item it{};
@@ -641,28 +562,6 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
     it.q_hi = min(it.q0 + tpc, it.n);
     it.kv_len = it.start + it.q_hi;
     it.ntiles = (it.kv_len + kN - 1) / kN;
-    if constexpr (MODE > 0) {
-      // whole warps get here
-      it.prefix = p.mod.prefix ? max(0, min(p.mod.prefix[it.b], ctx)) : 0;
-      it.head = max(it.prefix, p.mod.sink);
-      int lo = INT_MAX;
-      if (p.mod.first) {
-        for (int t = it.q0 + (threadIdx.x & 31); t < it.q_hi; t += 32)
-          lo = min(lo, p.mod.first[p.q_start[it.b] + t]);
-        lo = __reduce_min_sync(0xffffffffu, lo);
-      } else {
-        lo = 0;
-      }
-      // a bound only: the least of the rows' documents and the first row's window
-      it.lo = max(0, lo);
-      if (p.mod.window > 0) it.lo = max(it.lo, it.start + it.q0 - p.mod.window + 1);
-      const int last = it.kv_len - 1;  // last causal key of the item
-      it.kv_len = max(it.kv_len, it.prefix);
-      it.head_tiles = min((it.head + kN - 1) / kN, last / kN + 1);
-      // the tile of lo (or the last causal one) is read in any case
-      it.skip = max(0, min(it.lo, last) / kN - it.head_tiles);
-      it.ntiles = (it.kv_len + kN - 1) / kN - it.skip;
-    }
     it.ok = true;
     return it;
   };
@@ -723,12 +622,8 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
       const Item it = item_at(e);
       if (!it.ok) continue;
       const int b = it.b, h = it.h, kv_len = it.kv_len, ntiles = it.ntiles;
-      auto own = [&](int t) {  // the sequence's tile of local tile t
-        if constexpr (MODE > 0) return t < it.head_tiles ? t : t + it.skip;
-        return t;
-      };
       auto group_key = [&](int g) {
-        return lane < 4 * nst ? own(4 * g + (lane >> nst_log2)) * kN + (lane & (nst - 1)) * sub
+        return lane < 4 * nst ? (4 * g + (lane >> nst_log2)) * kN + (lane & (nst - 1)) * sub
                               : kv_len;
       };
       auto group_ids = [&](int g) -> int32_t {
@@ -739,14 +634,13 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
         const int t = group_key(g);
         if (t >= kv_len) return 0;
         if (blk < 0 || blk >= p.n_blocks) {
-          // (a box that no row sees may have lost its block: any block will do)
-          if (MODE == 0 || t < it.head || t + sub > it.lo) dev_error(p.err, MZ_DEVERR_BLOCK_ID);
+          dev_error(p.err, MZ_DEVERR_BLOCK_ID);
           blk = 0;
         }
         return static_cast<int>(((int64_t)blk * p.Hkv + h) * p.bs + t % p.bs);
       };
       auto load = [&](const CUtensorMap *tm, uint32_t dst, uint32_t fbar, int j, int y) {
-        const int nsub = min(nst, (kv_len - own(j) * kN + sub - 1) >> p.sub_log2);
+        const int nsub = min(nst, (kv_len - j * kN + sub - 1) >> p.sub_log2);
         if (lane == 0)
           mbar_arrive_expect_tx(fbar, static_cast<uint32_t>(nsub * (D / 64) * sub * 128));
         __syncwarp();
@@ -907,15 +801,6 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
       const int hq = it.h * p.G + row % p.G;
       const bool live = tok < q_hi;
       const int lim = start + min(tok, q_hi - 1);  // last visible key of the row
-      // MODE > 0: the row's lowest key, its keys [0, head) and its slope
-      int row_lo = 0, row_head = 0;
-      float slope = 0.f;
-      if constexpr (MODE > 0) {
-        if (p.mod.first) row_lo = max(0, p.mod.first[p.q_start[b] + min(tok, q_hi - 1)]);
-        if (p.mod.window > 0) row_lo = max(row_lo, lim - p.mod.window + 1);
-        row_head = max(it.prefix, min(p.mod.sink, lim + 1));
-        if (MODE > 1 && p.mod.slopes) slope = p.mod.slopes[hq] * kLog2e;
-      }
       {
         // half hf of the Q row -> shared memory (128-byte-swizzled K-major
         // layout); every S of the item before has completed (this thread
@@ -933,10 +818,9 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(bar(kBarQReady));
       }
-      float m_used = MODE > 0 ? kNoMax : -INFINITY, l = 0.f;
+      float m_used = -INFINITY, l = 0.f;
       for (int i = 0; i < ntiles; ++i) {
         const int g = tg + i;
-        const int tile = MODE > 0 && i >= it.head_tiles ? i + it.skip : i;  // the sequence's
         if (__any_sync(0xffffffffu, *abort_flag != 0)) {
           ok = false;
           break;
@@ -961,30 +845,8 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
   #pragma unroll
             for (int j = 0; j < 32; ++j) sv[32 * c + j] = __uint_as_float(r[c][j]);
         }
-        const int key0 = tile * kN + kH * hf;
-        if constexpr (MODE > 2) {
-#pragma unroll
-          for (int j = 0; j < kH; ++j) sv[j] = p.mod.cap_log2 * tanh_mod(sv[j] * p.mod.z_scale);
-        } else if constexpr (MODE > 1) {
-#pragma unroll
-          for (int j = 0; j < kH; ++j) sv[j] *= p.scale_log2;
-        }
-        if constexpr (MODE > 1) {
-          if (p.mod.slopes) {
-            const float d0 = static_cast<float>(key0 - lim);
-#pragma unroll
-            for (int j = 0; j < kH; ++j) sv[j] = fmaf(-slope, fabsf(d0 + j), sv[j]);
-          }
-        }
-        if constexpr (MODE > 0) {
-          if (!((key0 >= row_lo && key0 + kH - 1 <= lim) || key0 + kH <= row_head)) {
-#pragma unroll
-            for (int j = 0; j < kH; ++j) {
-              const int key = key0 + j;
-              if (key >= row_head && (key > lim || key < row_lo)) sv[j] = -INFINITY;
-            }
-          }
-        } else if (key0 + kH - 1 > lim) {  // this half crosses the row's causal limit
+        const int key0 = i * kN + kH * hf;
+        if (key0 + kH - 1 > lim) {  // this half crosses the row's causal limit
   #pragma unroll
           for (int j = 0; j < kH; ++j)
             if (key0 + j > lim) sv[j] = -INFINITY;
@@ -1012,8 +874,7 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
             ok = false;
             break;
           }
-          mx = fmaxf(xm[(par * 2) * kM + row], xm[(par * 2 + 1) * kM + row]);
-          if constexpr (MODE < 2) mx *= p.scale_log2;
+          mx = fmaxf(xm[(par * 2) * kM + row], xm[(par * 2 + 1) * kM + row]) * p.scale_log2;
         }
         const bool need = mx > m_used + kRescaleLog2;
         const float m_new = need ? mx : m_used;
@@ -1050,8 +911,7 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
   #pragma unroll
           for (int w = 0; w < 16; ++w) {
             float xa, xe;
-            const uint64_t s2 = f2_pack(sv[32 * c + 2 * w], sv[32 * c + 2 * w + 1]);
-            f2_unpack(MODE < 2 ? f2_fma(s2, sc2, nm2) : f2_add(s2, nm2), xa, xe);
+            f2_unpack(f2_fma(f2_pack(sv[32 * c + 2 * w], sv[32 * c + 2 * w + 1]), sc2, nm2), xa, xe);
             const float a = fast_exp2(xa), e = fast_exp2(xe);
             const uint64_t ae = f2_pack(a, e);
             l2[w & 3] = f2_add(l2[w & 3], ae);
@@ -1072,13 +932,10 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
   #pragma unroll
         for (int k = 0; k < 4; ++k) f2_unpack(l2[k], l8[2 * k], l8[2 * k + 1]);
         l = l * alpha + (((l8[0] + l8[1]) + (l8[2] + l8[3])) + ((l8[4] + l8[5]) + (l8[6] + l8[7])));
-        const int nvalid = kv_len - tile * kN;
-        // MODE > 0: the tile holds keys of the hole between head and lo
-        const bool hole = MODE > 0 && tile * kN < it.lo && (tile + 1) * kN > it.head;
-        if (nvalid < kN || hole) {
+        const int nvalid = kv_len - i * kN;
+        if (nvalid < kN) {
           // last tile: keys past kv_len hold stale smem / pool rows; their P is
-          // 0 but 0 * NaN is not, so the V rows become exact zeros first; the
-          // same for keys that no row of the item sees
+          // 0 but 0 * NaN is not, so the V rows become exact zeros first
           const int s = g % kVRing;
           if (!__all_sync(0xffffffffu,
                           mbar_wait_bounded(bar(kBarVFull + s), (g / kVRing) & 1, kTimeoutNs))) {
@@ -1086,15 +943,10 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
             ok = false;
             break;
           }
-          const int r0 = hole ? 0 : nvalid;
-          const int units = (kN - r0) * (D / 8);
+          const int units = (kN - nvalid) * (D / 8);
           for (int e = threadIdx.x; e < units; e += 32 * kSoftWarps) {
-            const int r = r0 + e / (D / 8), u = e % (D / 8);
+            const int r = nvalid + e / (D / 8), u = e % (D / 8);
             const int c = u >> 3, uu = u & 7;
-            if (hole) {
-              const int key = tile * kN + r;
-              if (key < kv_len && (key < it.head || key >= it.lo)) continue;
-            }
             *reinterpret_cast<uint4 *>(smem + C::kV0 + s * C::kTile + (r >> 3) * C::kGroup +
                                        c * 1024 + (r & 7) * 128 + ((uu ^ (r & 7)) << 4)) =
                 make_uint4(0, 0, 0, 0);
@@ -1121,8 +973,7 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
       }
       if (ok) {
         tc::fence_after_sync();
-        const float sum = xl[row] + xl[kM + row];
-        const float inv = MODE > 0 ? decode::row_inverse(sum) : 1.f / sum;
+        const float inv = 1.f / (xl[row] + xl[kM + row]);
         const int64_t ob = (int64_t)(p.q_start[b] + tok) * p.o_st + (int64_t)hq * p.o_sh;
   #pragma unroll
         for (int c = hf * (D / 64); c < (hf + 1) * (D / 64); ++c) {
@@ -1171,10 +1022,10 @@ __global__ void __launch_bounds__(tcp::kThreads, 1)
   }
 }
 
-template <int D, bool BF16, int MODE>
+template <int D, bool BF16>
 int smem_attr_ps() {
   static DeviceOnce once;
-  return smem_optin(paged_prefill_ps_kernel<D, BF16, MODE>, tcp::TCfg<D>::kSmemBytes, once,
+  return smem_optin(paged_prefill_ps_kernel<D, BF16>, tcp::TCfg<D>::kSmemBytes, once,
                     "mz_paged_prefill: shared memory attribute (persistent form)");
 }
 
@@ -1191,110 +1042,43 @@ int smem_attr_tc() {
 using namespace mz;
 using namespace mz::prefill;
 
-static int launch_prefill(void *out, int32_t out_dtype, int64_t out_tok_stride,
-                          int64_t out_head_stride, const void *q, int64_t q_tok_stride,
-                          int64_t q_head_stride, int32_t n_rows, const int32_t *q_start,
-                          const int32_t *q_len, int32_t max_q_len, const void *k_pool,
-                          const void *v_pool, const int32_t *block_tables,
-                          int32_t max_blocks_per_seq, const int32_t *ctx_lens, int32_t n_seqs,
-                          int32_t n_heads, int32_t n_kv_heads, int32_t head_dim,
-                          int32_t block_size, int64_t n_blocks, float scale, int32_t dtype,
-                          int32_t *dev_err, mz_stream_t stream, const char *fn,
-                          const mz_score_mod *mod) {
-  if (dtype != MZ_DTYPE_F16 && dtype != MZ_DTYPE_BF16)
-    return fail(MZ_ERR_UNSUPPORTED, "%s: dtype must be F16 or BF16", fn);
-  if (out_dtype != dtype && out_dtype != MZ_DTYPE_F32)
-    return fail(MZ_ERR_UNSUPPORTED, "%s: out_dtype must equal dtype or be F32", fn);
-  if (head_dim != 64 && head_dim != 128)
-    return fail(MZ_ERR_UNSUPPORTED, "%s: head_dim %d (supported: 64, 128)", fn, head_dim);
-  if (block_size <= 0 || block_size % kTileTok)
-    return fail(MZ_ERR_UNSUPPORTED, "%s: block_size %d is not a multiple of 16", fn, block_size);
-  if (n_seqs < 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || max_q_len < 0 ||
-      max_blocks_per_seq <= 0 || n_blocks <= 0 || n_rows < 0)
-    return fail(MZ_ERR_INVALID_ARG, "%s: bad sizes", fn);
-  const int G = n_heads / n_kv_heads;
-  if (tcp::kM % G)
-    return fail(MZ_ERR_UNSUPPORTED, "%s: n_heads / n_kv_heads = %d does not divide %d", fn, G,
-                tcp::kM);
-  if (!std::isfinite(scale) || !(scale > 0.f))
-    return fail(MZ_ERR_INVALID_ARG, "%s: scale must be finite and positive", fn);
-  if (n_seqs == 0 || max_q_len == 0) return MZ_OK;
-  if (!out || !q || !q_start || !q_len || !k_pool || !v_pool || !block_tables || !ctx_lens)
-    return fail(MZ_ERR_INVALID_ARG, "%s: null pointer", fn);
-  // rows move as 16-byte vectors: q and out 16-byte aligned, strides whole vectors
-  const int oe = out_dtype == MZ_DTYPE_F32 ? 4 : 8;
-  if (!aligned(k_pool, 16) || !aligned(v_pool, 16) || !aligned(q, 16) || (q_tok_stride % 8) ||
-      (q_head_stride % 8) || !aligned(out, 16) || (out_tok_stride % oe) || (out_head_stride % oe))
-    return fail(MZ_ERR_ALIGNMENT,
-                "%s: pools, q and out need 16-byte alignment and strides of whole 16-byte "
-                "vectors", fn);
-  const int64_t rows_total = n_blocks * n_kv_heads * block_size;
-  if (rows_total >= (int64_t(1) << 31))
-    return fail(MZ_ERR_UNSUPPORTED, "%s: pool has >= 2^31 rows", fn);
-
-  const bool bf16 = dtype == MZ_DTYPE_BF16;
+extern "C" int mz_paged_prefill(void *out, int32_t out_dtype, int64_t out_tok_stride,
+                                int64_t out_head_stride, const void *q, int64_t q_tok_stride,
+                                int64_t q_head_stride, int32_t n_rows, const int32_t *q_start,
+                                const int32_t *q_len, int32_t max_q_len, const void *k_pool,
+                                const void *v_pool, const int32_t *block_tables,
+                                int32_t max_blocks_per_seq, const int32_t *ctx_lens,
+                                int32_t n_seqs, int32_t n_heads, int32_t n_kv_heads,
+                                int32_t head_dim, int32_t block_size, int64_t n_blocks,
+                                float scale, int32_t dtype, int32_t *dev_err,
+                                mz_stream_t stream) {
+  const char *fn = "mz_paged_prefill";
   CUtensorMap tk, tv;
-  const auto type = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  int sub_log2 = 4;  // rows per copy box: gcd(block_size, 128)
-  while (sub_log2 < 7 && block_size % (1 << (sub_log2 + 1)) == 0) ++sub_log2;
-  if (int rc = make_group_map(&tk, k_pool, rows_total, head_dim, type, 1 << sub_log2)) return rc;
-  if (int rc = make_group_map(&tv, v_pool, rows_total, head_dim, type, 1 << sub_log2)) return rc;
-
   PParams p;
-  p.out = out;
-  p.o_st = out_tok_stride;
-  p.o_sh = out_head_stride;
-  p.out_f32 = out_dtype == MZ_DTYPE_F32;
-  p.q = q;
-  p.q_st = q_tok_stride;
-  p.q_sh = q_head_stride;
-  p.n_rows = n_rows;
-  p.q_start = q_start;
-  p.q_len = q_len;
-  p.ctx = ctx_lens;
-  p.tables = block_tables;
-  p.max_blocks = max_blocks_per_seq;
-  p.Hkv = n_kv_heads;
-  p.G = G;
-  p.bs = block_size;
-  p.n_blocks = n_blocks;
-  p.scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
-  p.sub_log2 = sub_log2;
-  p.err = dev_err;
-  int mode = 0;
-  if (mod) {
-    if (int rc = make_score_mod(&p.mod, mod, scale, (int64_t)max_blocks_per_seq * block_size, fn))
-      return rc;
-    mode = p.mod.z_scale != 0.f ? 3 : p.mod.slopes ? 2 : 1;
-  }
+  bool empty = false;
+  if (int rc = prepare(&p, &tk, &tv, &empty, 7, out, out_dtype, out_tok_stride, out_head_stride, q,
+                       q_tok_stride, q_head_stride, n_rows, q_start, q_len, max_q_len, k_pool,
+                       v_pool, block_tables, max_blocks_per_seq, ctx_lens, n_seqs, n_heads,
+                       n_kv_heads, head_dim, block_size, n_blocks, scale, dtype, dev_err, fn))
+    return rc;
+  if (empty) return MZ_OK;
 
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (n_seqs > 65535 || n_kv_heads > 65535)
-    return fail(MZ_ERR_UNSUPPORTED, "%s: grid too large", fn);
-  const int tpc = tcp::kM / G;
+  const int tpc = kM / (n_heads / n_kv_heads);
+  const bool bf16 = dtype == MZ_DTYPE_BF16;
   // The persistent form (one CTA per SM over all query blocks) by default;
   // MLXZ_B200_PREFILL_PERSIST=0 launches one CTA per query block instead
-  // (modified scores and masks have the persistent form alone)
-  if (mode > 0 || decode::env_int("MLXZ_B200_PREFILL_PERSIST", 1, 0, 1) == 1) {
-    p.n_seqs = n_seqs;
-    p.qblocks = (max_q_len + tpc - 1) / tpc;
+  if (decode::env_int("MLXZ_B200_PREFILL_PERSIST", 1, 0, 1) == 1) {
     const int64_t items = (int64_t)n_seqs * n_kv_heads * p.qblocks;
     if (items >= (int64_t(1) << 31)) return fail(MZ_ERR_UNSUPPORTED, "%s: too many query blocks", fn);
     const int sms = sm_count(current_device());
     if (sms <= 0) return fail(MZ_ERR_CUDA, "%s: cannot query the SM count", fn);
     const dim3 grid_ps(static_cast<unsigned>(std::min<int64_t>(items, sms)));
-#define MZ_PSMODE(D_, BF_, MODE_)                                                                \
-  do {                                                                                           \
-    if (int rc = smem_attr_ps<D_, BF_, MODE_>()) return rc;                                      \
-    paged_prefill_ps_kernel<D_, BF_, MODE_>                                                      \
-        <<<grid_ps, tcp::kThreads, tcp::TCfg<D_>::kSmemBytes, s>>>(tk, tv, p);                   \
-  } while (0)
 #define MZ_PSLAUNCH(D_, BF_)                                                                     \
   do {                                                                                           \
-    if (mode == 0) MZ_PSMODE(D_, BF_, 0);                                                        \
-    else if (mode == 1) MZ_PSMODE(D_, BF_, 1);                                                   \
-    else if (mode == 2) MZ_PSMODE(D_, BF_, 2);                                                   \
-    else MZ_PSMODE(D_, BF_, 3);                                                                  \
+    if (int rc = smem_attr_ps<D_, BF_>()) return rc;                                             \
+    paged_prefill_ps_kernel<D_, BF_>                                                             \
+        <<<grid_ps, tcp::kThreads, tcp::TCfg<D_>::kSmemBytes, s>>>(tk, tv, p);                   \
   } while (0)
     if (head_dim == 128) {
       if (bf16) MZ_PSLAUNCH(128, true); else MZ_PSLAUNCH(128, false);
@@ -1302,7 +1086,6 @@ static int launch_prefill(void *out, int32_t out_dtype, int64_t out_tok_stride,
       if (bf16) MZ_PSLAUNCH(64, true); else MZ_PSLAUNCH(64, false);
     }
 #undef MZ_PSLAUNCH
-#undef MZ_PSMODE
     MZ_CHECK_LAUNCH(fn);
     return MZ_OK;
   }
@@ -1321,38 +1104,4 @@ static int launch_prefill(void *out, int32_t out_dtype, int64_t out_tok_stride,
 #undef MZ_TCLAUNCH
   MZ_CHECK_LAUNCH(fn);
   return MZ_OK;
-}
-
-extern "C" int mz_paged_prefill(void *out, int32_t out_dtype, int64_t out_tok_stride,
-                                int64_t out_head_stride, const void *q, int64_t q_tok_stride,
-                                int64_t q_head_stride, int32_t n_rows, const int32_t *q_start,
-                                const int32_t *q_len, int32_t max_q_len, const void *k_pool,
-                                const void *v_pool, const int32_t *block_tables,
-                                int32_t max_blocks_per_seq, const int32_t *ctx_lens,
-                                int32_t n_seqs, int32_t n_heads, int32_t n_kv_heads,
-                                int32_t head_dim, int32_t block_size, int64_t n_blocks,
-                                float scale, int32_t dtype, int32_t *dev_err,
-                                mz_stream_t stream) {
-  return launch_prefill(out, out_dtype, out_tok_stride, out_head_stride, q, q_tok_stride, q_head_stride,
-                 n_rows, q_start, q_len, max_q_len, k_pool, v_pool, block_tables,
-                 max_blocks_per_seq, ctx_lens, n_seqs, n_heads, n_kv_heads, head_dim, block_size,
-                 n_blocks, scale, dtype, dev_err, stream, "mz_paged_prefill", nullptr);
-}
-
-extern "C" int mz_paged_prefill_mod(void *out, int32_t out_dtype, int64_t out_tok_stride,
-                                    int64_t out_head_stride, const void *q, int64_t q_tok_stride,
-                                    int64_t q_head_stride, int32_t n_rows, const int32_t *q_start,
-                                    const int32_t *q_len, int32_t max_q_len, const void *k_pool,
-                                    const void *v_pool, const int32_t *block_tables,
-                                    int32_t max_blocks_per_seq, const int32_t *ctx_lens,
-                                    int32_t n_seqs, int32_t n_heads, int32_t n_kv_heads,
-                                    int32_t head_dim, int32_t block_size, int64_t n_blocks,
-                                    float scale, const mz_score_mod *mod, int32_t dtype,
-                                    int32_t *dev_err, mz_stream_t stream) {
-  const char *fn = "mz_paged_prefill_mod";
-  if (!mod) return fail(MZ_ERR_INVALID_ARG, "%s: mod is null", fn);
-  return launch_prefill(out, out_dtype, out_tok_stride, out_head_stride, q, q_tok_stride, q_head_stride,
-                 n_rows, q_start, q_len, max_q_len, k_pool, v_pool, block_tables,
-                 max_blocks_per_seq, ctx_lens, n_seqs, n_heads, n_kv_heads, head_dim, block_size,
-                 n_blocks, scale, dtype, dev_err, stream, fn, mod);
 }
