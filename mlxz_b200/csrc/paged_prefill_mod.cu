@@ -11,15 +11,20 @@
 //   a copy warp          streams 64-key K and V tiles through the block table
 //                        (bulk tensor copies of gcd(block_size, 64)-row boxes,
 //                        128-byte swizzle, no multicast), two slots of each
-//   an MMA warp          S_i = Q.K_i^T (SS, M = 128, N = 64) into S buffer i % 2,
-//                        then O += P_{i-1}.V_{i-1} (TS, N = D)
-// What bounds it: the scores of a tile pass the special-function unit (one
-// exponential each, three with a cap outside the polynomial's range) and about
-// five fp32 and conversion instructions each, in dependent phases with waits
-// between them; the MMAs of 128 keys (bf16's P.V twice, for the high and the
-// low part of P) take about 1800 cycles.  One stream alone leaves each idle
-// while the other works; two streams without any order between them fill each
-// other's gaps, and S of the next tile is computed during the softmax of this.
+//   an MMA warp          S_{i+1} = Q.K_{i+1}^T (SS, M = 128, N = 64) into S buffer
+//                        (i + 1) % 2, then O += P_i.V_i (TS, N = D)
+// What bounds it: a softmax warp's 64 scores a thread take about 1500 cycles a
+// tile, in dependent phases (TMEM load, maximum, exponentials, conversion, TMEM
+// store), of which the special-function unit needs 512; two warps of two streams
+// share a scheduler, and two streams without any order between them fill each
+// other's gaps: 4096 new tokens at 16384 with a window of 4096 (32 / 8 heads of
+// 128, bf16) take 357 us, 770 TFLOP/s, against 418 us for one stream of 128-key
+// tiles whose halves meet at every maximum.  Not kept, each right but slower on
+// that case: P.V issued apart from S, by a second warp (533 us) or by one warp
+// that polls both streams' barriers (425 us with S first, 482 us with P.V first);
+// the MMAs issued by one lane's branch instead of an elected lane (414 us);
+// exponentials against the running maximum as it is while the tile's is found,
+// redone where it moves (365 us).  P in one bf16 part would give 321 us.
 //
 // TMEM columns of stream s: O at 128 s, S buffers at 256 + 128 s, 64 each.  P
 // takes its scores' place: hi parts in the first 32 columns, lo in the last.
@@ -48,6 +53,7 @@ constexpr int kSoftWarps = 4;  // per stream
 constexpr int kThreads = 32 * kStreams * (kSoftWarps + 2);
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleLog2 = 8.f;
+constexpr int kPairs = 8;
 static_assert(kSlots == 2, "phases below count tiles by pairs");
 
 template <int D>
@@ -76,11 +82,15 @@ struct Item {
   __device__ __forceinline__ int own(int t) const { return t < head_tiles ? t : t + skip; }
 };
 
-// Item e, whole warps: query block qblocks - 1 - e % qblocks (a pair's longest
-// first) of pair e / qblocks = (sequence, KV head).  False: nothing to do.
+// Item e, whole warps: a query block (the last, longest ones first) of a pair =
+// (sequence, KV head).  False: nothing to do.
 __device__ __forceinline__ bool item_at(const PParams &p, int e, Item &it) {
   const int lane = threadIdx.x & 31, tpc = kM / p.G;
-  const int pair = e / p.qblocks, jr = e - pair * p.qblocks;
+  // kPairs pairs at a time, their query blocks in turn: neighbours in time share
+  // K/V through L2 without all reading the same tiles at once
+  const int pairs = p.n_seqs * p.Hkv;
+  const int first = e / (kPairs * p.qblocks) * kPairs, np = min(kPairs, pairs - first);
+  const int r = e - first * p.qblocks, jr = r / np, pair = first + r - jr * np;
   it.b = pair / p.Hkv;
   it.h = pair - it.b * p.Hkv;
   it.q0 = (p.qblocks - 1 - jr) * tpc;
@@ -116,11 +126,22 @@ __device__ __forceinline__ bool item_at(const PParams &p, int e, Item &it) {
   return true;
 }
 
-// tanh(z) = z P(z^2) for |z| <= 1/2: the polynomial that equals tanh(z) / z at the
-// five Chebyshev nodes of [0, 1/4] in z^2, within 6e-9.
-constexpr float kTanhRange = 0.5f;
-constexpr float kT0 = 1.0f, kT1 = -0.33333069f, kT2 = 0.13324751f, kT3 = -0.052984238f,
-                kT4 = 0.017131345f;
+// mbar_wait_bounded that also ends, every so many polls, when a role gave up.
+__device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t phase,
+                                             const volatile int *abort_flag) {
+  uint64_t t0 = 0;
+  for (uint32_t it = 1;; ++it) {
+    if (mbar_try_wait(bar, phase)) return true;
+    if ((it & 255u) == 0u) {
+      if (*abort_flag) return false;
+      const uint64_t now = global_timer_ns();
+      if (t0 == 0)
+        t0 = now;
+      else if (now - t0 > kTimeoutNs)
+        return false;
+    }
+  }
+}
 
 __device__ __forceinline__ float rcp_approx(float x) {
   float y;
@@ -182,13 +203,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     dev_error(p.err, MZ_DEVERR_TIMEOUT);
     *abort_flag = 1;
   };
-  // whole warp: barrier b of tile pair phase; false when it (or another role) gave up
+  // whole warp: phase `phase` of barrier b; false when it (or another role) gave up
   auto wait = [&](int b, int phase) {
-    if (__all_sync(0xffffffffu, mbar_wait_bounded(bar(b), phase & 1, kTimeoutNs))) return true;
+    if (__all_sync(0xffffffffu, wait_bounded(bar(b), phase & 1, abort_flag))) return true;
     if (lane == 0) give_up();
     return false;
   };
-  auto aborted = [&]() { return __any_sync(0xffffffffu, *abort_flag != 0) != 0; };
 
   Item it;
   int g = 0;  // tiles of this stream so far: slot g % 2, barrier phase g / 2
@@ -231,10 +251,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       int y_prev = 0, y_cur = rows(0, ids(0));
       int32_t id_next = ids(1);
       for (int t = 0; t <= it.ntiles; ++t) {
-        if (aborted()) {
-          ok = false;
-          break;
-        }
         if (t > 0 && t % per == 0) {
           y_prev = y_cur;
           y_cur = rows(t / per, id_next);
@@ -302,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         break;
       }
       for (int i = 0; i < it.ntiles; ++i) {
-        if (aborted() || (i + 1 < it.ntiles && !issue_s(g + i + 1))) {
+        if (i + 1 < it.ntiles && !issue_s(g + i + 1)) {
           ok = false;
           break;
         }
@@ -367,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool have2 = false;
       for (int i = 0; i < it.ntiles; ++i) {
         const int j = g + i, s = j & 1, tile = it.own(i);
-        if (aborted() || !wait(kBarSFull + s, j >> 1)) {
+        if (!wait(kBarSFull + s, j >> 1)) {
           ok = false;
           break;
         }
@@ -387,26 +403,22 @@ __global__ void __launch_bounds__(kThreads, 1)
           float big = fmax3f(fabsf(sv[0]), fabsf(sv[1]), 0.f);
 #pragma unroll
           for (int x = 2; x < kN; x += 2) big = fmax3f(big, fabsf(sv[x]), fabsf(sv[x + 1]));
-          if (__any_sync(0xffffffffu, !(big * p.mod.z_scale <= kTanhRange))) {
+          if (__any_sync(0xffffffffu, !(big <= p.mod.poly_range))) {
             // cap - 2 cap / (e^(2 z) + 1)
             const float k2 = p.mod.z_scale * (2.f * kLog2e), c2 = -2.f * p.mod.cap_log2;
 #pragma unroll
             for (int x = 0; x < kN; ++x)
               sv[x] = fmaf(c2, rcp_approx(fast_exp2(sv[x] * k2) + 1.f), p.mod.cap_log2);
           } else {
-            const float c = p.mod.cap_log2;
-            const uint64_t zs = f2_pack(p.mod.z_scale, p.mod.z_scale);
-            const uint64_t c0 = f2_pack(kT0 * c, kT0 * c), c1 = f2_pack(kT1 * c, kT1 * c),
-                           c2 = f2_pack(kT2 * c, kT2 * c), c3 = f2_pack(kT3 * c, kT3 * c),
-                           c4 = f2_pack(kT4 * c, kT4 * c);
+            const uint64_t c0 = f2_pack(p.mod.poly[0], p.mod.poly[0]),
+                           c1 = f2_pack(p.mod.poly[1], p.mod.poly[1]),
+                           c2 = f2_pack(p.mod.poly[2], p.mod.poly[2]),
+                           c3 = f2_pack(p.mod.poly[3], p.mod.poly[3]);
 #pragma unroll
             for (int x = 0; x < kN; x += 2) {
-              const uint64_t z = f2_mul(f2_pack(sv[x], sv[x + 1]), zs), w = f2_mul(z, z);
-              uint64_t y = f2_fma(w, c4, c3);
-              y = f2_fma(y, w, c2);
-              y = f2_fma(y, w, c1);
-              y = f2_fma(y, w, c0);
-              f2_unpack(f2_mul(y, z), sv[x], sv[x + 1]);
+              const uint64_t v = f2_pack(sv[x], sv[x + 1]), w = f2_mul(v, v);
+              const uint64_t y = f2_fma(f2_fma(f2_fma(w, c3, c2), w, c1), w, c0);
+              f2_unpack(f2_mul(y, v), sv[x], sv[x + 1]);
             }
           }
         }
