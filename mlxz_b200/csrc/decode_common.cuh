@@ -133,9 +133,13 @@ struct MaskSpan {
   int prefix, head, lo;
 };
 
+__device__ __forceinline__ int mask_prefix(const ModParams &p, int b, int ctx) {
+  return p.mod.prefix ? max(0, min(p.mod.prefix[b], ctx)) : 0;
+}
+
 __device__ __forceinline__ MaskSpan mask_span(const ModParams &p, int b, int ctx) {
   MaskSpan s;
-  s.prefix = p.mod.prefix ? max(0, min(p.mod.prefix[b], ctx)) : 0;
+  s.prefix = mask_prefix(p, b, ctx);
   s.head = max(s.prefix, p.mod.sink);
   s.lo = p.mod.first ? max(0, p.mod.first[b]) : 0;
   if (p.mod.window > 0) s.lo = max(s.lo, ctx - p.n_q - p.mod.window + 1);
@@ -157,7 +161,7 @@ __device__ __forceinline__ int own_tile(const Params &, int, int t, int, int) { 
 __device__ __forceinline__ int own_tile(const ModParams &p, int b, int t, int n, int ctx) {
   const int skip = ntiles_of(ctx) - n;
   if (skip == 0) return t;
-  return t < ntiles_of(mask_span(p, b, ctx).head) ? t : t + skip;
+  return t < ntiles_of(max(mask_prefix(p, b, ctx), p.mod.sink)) ? t : t + skip;
 }
 
 template <class P>

@@ -244,28 +244,59 @@ __device__ __forceinline__ void decode_tiles(const CUtensorMap &tmK, const CUten
 
     // Online softmax (exp2 domain), rows g (regs 0,1) and g+8 (regs 2,3).
     float mx0 = -INFINITY, mx1 = -INFINITY;
-    // MOD: every row sees every key of the tile
-    const bool all_seen = MOD && key0 >= lo_max && key0 + kTileTok - 1 <= p_min;
+    if constexpr (MOD) {
+      // rows g + 8 only where there are any
+      const int ne = two_groups ? 4 : 2;
+      if (p.mod.z_scale == 0.f) {
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+        for (int x = 0; x < 8; ++x)
+          if ((x & 3) < ne) sacc[x >> 2][x & 3] *= p.scale_log2;
+      } else if (p.mod.cap_log2 <= kQuickCapLog2) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int tok = n * 8 + 2 * cq + (e & 1);
-        float x = sacc[n][e] * p.scale_log2;
-        if constexpr (MOD) {
-          const int key = key0 + tok, pos = e < 2 ? pos0 : pos1, lo = e < 2 ? lo0 : lo1;
-          if (p.mod.z_scale != 0.f) x = p.mod.cap_log2 * tanh_mod(sacc[n][e] * p.mod.z_scale);
-          if (p.mod.slopes)
-            x = fmaf(-(e < 2 ? slope0 : slope1), fabsf(static_cast<float>(pos - key)), x);
-          if (!all_seen && !(key < span.prefix ||
-                             (key <= pos && (key >= lo || key < p.mod.sink))))
-            x = -INFINITY;
-        } else {
-          if (tok >= nvalid) x = -INFINITY;
-        }
-        sacc[n][e] = x;
-        if (e < 2) mx0 = fmaxf(mx0, x); else mx1 = fmaxf(mx1, x);
+        for (int x = 0; x < 8; ++x)
+          if ((x & 3) < ne) sacc[x >> 2][x & 3] = cap_quick(p.mod, sacc[x >> 2][x & 3]);
+      } else {
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+          if ((x & 3) < ne)
+            sacc[x >> 2][x & 3] =
+                p.mod.cap_log2 * tanh_mod(sacc[x >> 2][x & 3] * p.mod.z_scale);
       }
+      if (p.mod.slopes) {
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const int key = key0 + (x >> 2) * 8 + 2 * cq + (x & 1);
+          const float far = static_cast<float>(((x & 2) ? pos1 : pos0) - key);
+          sacc[x >> 2][x & 3] = fmaf(-((x & 2) ? slope1 : slope0), fabsf(far), sacc[x >> 2][x & 3]);
+        }
+      }
+      // not every row sees every key of the tile
+      if (!((key0 >= lo_max && key0 + kTileTok - 1 <= p_min) || key0 + kTileTok <= span.prefix)) {
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+          const int key = key0 + (x >> 2) * 8 + 2 * cq + (x & 1);
+          const int pos = (x & 2) ? pos1 : pos0, lo = (x & 2) ? lo1 : lo0;
+          if (!(key < span.prefix || (key <= pos && (key >= lo || key < p.mod.sink))))
+            sacc[x >> 2][x & 3] = -INFINITY;
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        mx0 = fmaxf(mx0, fmaxf(sacc[n][0], sacc[n][1]));
+        mx1 = fmaxf(mx1, fmaxf(sacc[n][2], sacc[n][3]));
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int tok = n * 8 + 2 * cq + (e & 1);
+          float x = sacc[n][e] * p.scale_log2;
+          if (tok >= nvalid) x = -INFINITY;
+          sacc[n][e] = x;
+          if (e < 2) mx0 = fmaxf(mx0, x); else mx1 = fmaxf(mx1, x);
+        }
+    }
     mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
     mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
     const float mn0 = fmaxf(m0, mx0);

@@ -143,12 +143,6 @@ __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t phase,
   }
 }
 
-__device__ __forceinline__ float rcp_approx(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // MODE 1: masks; 2: masks and the bias by distance; 3: these and capped scores.
 // From 2 on the scores take their final form, in log2 units, in registers.
 template <int D, bool BF16, int MODE>
@@ -404,11 +398,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int x = 2; x < kN; x += 2) big = fmax3f(big, fabsf(sv[x]), fabsf(sv[x + 1]));
           if (__any_sync(0xffffffffu, !(big <= p.mod.poly_range))) {
-            // cap - 2 cap / (e^(2 z) + 1)
-            const float k2 = p.mod.z_scale * (2.f * kLog2e), c2 = -2.f * p.mod.cap_log2;
 #pragma unroll
-            for (int x = 0; x < kN; ++x)
-              sv[x] = fmaf(c2, rcp_approx(fast_exp2(sv[x] * k2) + 1.f), p.mod.cap_log2);
+            for (int x = 0; x < kN; ++x) sv[x] = cap_quick(p.mod, sv[x]);
           } else {
             const uint64_t c0 = f2_pack(p.mod.poly[0], p.mod.poly[0]),
                            c1 = f2_pack(p.mod.poly[1], p.mod.poly[1]),
