@@ -62,7 +62,8 @@ def _dev_index(t: torch.Tensor) -> int:
 
 
 def _stream(device: int) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # the raw handle, without building a torch.cuda.Stream (2 us a call)
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def error_word(device: int) -> torch.Tensor:
@@ -98,14 +99,21 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 
 
 def _call(device: int, name: str, *args) -> None:
-    """nat.call with ``device`` current: a launch goes to the current device,
-    which need not be the tensors' own."""
-    if torch.cuda.current_device() == device:
-        nat.call(name, *args, error_word(device).data_ptr(), _stream(device))
+    """nat.call with the error word and the current stream behind ``args``, and
+    ``device`` current: a launch goes to the current device, which need not be
+    the tensors' own."""
+    err = error_word(device).data_ptr()
+    if torch._C._cuda_getDevice() == device:
+        nat.call(name, *args, err, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            nat.call(name, *args, error_word(device).data_ptr(), _stream(device))
-    _after(device)
+            nat.call(name, *args, err, _stream(device))
+    if _DEBUG:
+        check_device_errors(device)
+
+
+def _i32_on(t: torch.Tensor, dev: int) -> bool:
+    return t.dtype is torch.int32 and t.get_device() == dev and t.is_contiguous()
 
 
 def _check_pools(k_pool: torch.Tensor, v_pool: torch.Tensor) -> tuple[int, int, int, int]:
@@ -253,22 +261,22 @@ def paged_plan(block_tables: torch.Tensor, ctx_lens: torch.Tensor, q_lens: torch
     ``n_blocks``: blocks of the pools (bounds the ids)."""
     if block_tables.dim() != 2:
         raise ValueError("block_tables must be [B, max_blocks]")
-    device = block_tables.device
-    _as_i32(block_tables, device, "block_tables")
+    dev = block_tables.get_device()
     B, width = block_tables.shape
+    if not _i32_on(block_tables, dev):
+        _as_i32(block_tables, block_tables.device, "block_tables")
     for t, name in ((ctx_lens, "ctx_lens"), (q_lens, "q_lens"), (held, "held")):
-        if t is not None:
-            _as_i32(t, device, name)
-            if t.numel() != B:
-                raise ValueError(f"{name} must hold one entry per sequence ({B})")
-    if new_ids is not None:
-        _as_i32(new_ids, device, "new_ids")
+        if t is not None and not (_i32_on(t, dev) and t.numel() == B):
+            _as_i32(t, block_tables.device, name)
+            raise ValueError(f"{name} must hold one entry per sequence ({B})")
+    if new_ids is not None and not _i32_on(new_ids, dev):
+        _as_i32(new_ids, block_tables.device, "new_ids")
     if n_rows < 0 or block_size < 1 or n_blocks < 1:
         raise ValueError("n_rows must be >= 0, block_size and n_blocks >= 1")
     dev = _dev_index(block_tables)
-    positions, q_start, lengths, held_out, n_new = torch.empty(
-        n_rows + 3 * B + 1, dtype=torch.int32, device=device).split_with_sizes((n_rows, B, B, B, 1))
-    slots = torch.empty(n_rows, dtype=torch.int64, device=device)
+    positions, q_start, lengths, held_out, n_new = block_tables.new_empty(
+        n_rows + 3 * B + 1).split_with_sizes((n_rows, B, B, B, 1))
+    slots = block_tables.new_empty(n_rows, dtype=torch.int64)
     _call(dev, "mz_paged_plan", block_tables.data_ptr(), max(width, 1), ctx_lens.data_ptr(),
           q_lens.data_ptr(), _ptr(held), _ptr(new_ids), 0 if new_ids is None else new_ids.numel(),
           B, n_rows, block_size, n_blocks, q_start.data_ptr(), positions.data_ptr(),
@@ -280,44 +288,60 @@ def paged_plan(block_tables: torch.Tensor, ctx_lens: torch.Tensor, q_lens: torch
 # Query / key norm, rotation and append
 # ---------------------------------------------------------------------------
 
-def _rope_args(q, k, positions, inv_freq, q_weight, k_weight, eps, weight_offset, interleaved,
+def _rope_args(q, positions, inv_freq, q_weight, k_weight, eps, weight_offset, interleaved,
                freq_axes):
-    """Checks shared by the norm-and-rotation calls; the trailing arguments of
+    """Checks shared by the norm-and-rotation calls; the arguments of
     mz_qk_norm_rope from ``positions`` to ``norm``."""
-    T, Hq, D = q.shape
-    device = q.device
-    _as_i32(positions, device, "positions")
-    n_axes = 1 if positions.dim() == 1 else positions.shape[0]
-    if positions.dim() > 2 or positions.shape[-1] != T:
+    T, _, D = q.shape
+    dev = q.get_device()
+    if not _i32_on(positions, dev):
+        _as_i32(positions, q.device, "positions")
+    axes = positions.shape
+    n_axes = 1 if len(axes) == 1 else axes[0]
+    if len(axes) not in (1, 2) or axes[-1] != T:
         raise ValueError(f"positions must be int32 [{T}] or [axes, {T}]")
-    if inv_freq.dtype != torch.float32 or inv_freq.dim() != 1 or inv_freq.device != device or \
-            not inv_freq.is_contiguous():
-        raise ValueError(f"inv_freq must be a contiguous 1-D float32 tensor on {device}")
+    if inv_freq.dtype is not torch.float32 or inv_freq.dim() != 1 or \
+            inv_freq.get_device() != dev or not inv_freq.is_contiguous():
+        raise ValueError(f"inv_freq must be a contiguous 1-D float32 tensor on {q.device}")
     half = inv_freq.numel()
     if freq_axes is not None:
-        _as_i32(freq_axes, device, "freq_axes")
+        if not _i32_on(freq_axes, dev):
+            _as_i32(freq_axes, q.device, "freq_axes")
         if freq_axes.numel() != half:
             raise ValueError("freq_axes must name one position axis per frequency")
     elif n_axes > 1 and half:
         raise ValueError("several position axes need freq_axes")
-    w = q_weight if q_weight is not None else k_weight
-    if w is not None and eps is None:
-        raise ValueError("norm weights need eps")
+    w_dtype = None
     for x in (q_weight, k_weight):
-        if x is not None and (x.shape != (D,) or x.dtype != w.dtype or x.device != device
-                              or not x.is_contiguous()):
-            raise ValueError(f"norm weights must be contiguous [{D}] of one dtype on {device}")
+        if x is None:
+            continue
+        if eps is None:
+            raise ValueError("norm weights need eps")
+        if w_dtype is None:
+            w_dtype = x.dtype
+        if x.dtype is not w_dtype or x.shape != (D,) or x.get_device() != dev or \
+                not x.is_contiguous():
+            raise ValueError(f"norm weights must be contiguous [{D}] of one dtype on {q.device}")
     return (positions.data_ptr(), T, n_axes, inv_freq.data_ptr(), _ptr(freq_axes), 2 * half,
             1 if interleaved else 0, _ptr(q_weight), _ptr(k_weight),
-            0 if w is None else dtype_code(w.dtype), float(weight_offset),
-            0.0 if eps is None else float(eps), 0 if eps is None else 1)
+            0 if w_dtype is None else dtype_code(w_dtype), weight_offset,
+            0.0 if eps is None else eps, 0 if eps is None else 1)
 
 
-def _check_heads(t: torch.Tensor, name: str, like: torch.Tensor) -> None:
-    if t.dim() != 3 or t.shape[0] != like.shape[0] or t.shape[2] != like.shape[2] or \
-            t.stride(2) != 1 or t.dtype != like.dtype or t.device != like.device:
-        raise ValueError(f"{name} must be [{like.shape[0]}, heads, {like.shape[2]}] of "
-                         f"{like.dtype} on {like.device} with unit last stride")
+def _heads(t: torch.Tensor, name: str, like: torch.Tensor, n_heads: int | None = None
+           ) -> tuple[int, int, int]:
+    """(pointer, token stride, head stride) of a tensor ``[T, heads, D]`` like
+    ``like`` in all but the heads."""
+    shape, want = t.shape, like.shape
+    if len(shape) == 3 and shape[0] == want[0] and shape[2] == want[2] and \
+            t.dtype is like.dtype and t.get_device() == like.get_device() and \
+            (n_heads is None or shape[1] == n_heads):
+        ts, hs, one = t.stride()
+        if one == 1:
+            return t.data_ptr(), ts, hs
+    heads = "heads" if n_heads is None else f"{n_heads} heads"
+    raise ValueError(f"{name} must be [{want[0]}, {heads}, {want[2]}] of {like.dtype} on "
+                     f"{like.device} with unit last stride")
 
 
 def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
@@ -336,23 +360,20 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
     ``(i, i + len(inv_freq))`` or, ``interleaved``, ``(2i, 2i + 1)``.  The norm
     runs if ``eps`` is given, times ``weight + weight_offset`` where a weight
     is.  ``q_out`` / ``k_out`` may be q / k themselves."""
-    if q.dim() != 3 or q.stride(2) != 1:
+    if q.dim() != 3:
         raise ValueError("q must be [T, heads, D] with unit last stride")
-    _check_heads(k, "k", q)
-    args = _rope_args(q, k, positions, inv_freq, q_weight, k_weight, eps, weight_offset,
-                      interleaved, freq_axes)
+    q_at, k_at = _heads(q, "q", q), _heads(k, "k", q)
+    args = _rope_args(q, positions, inv_freq, q_weight, k_weight, eps, weight_offset, interleaved,
+                      freq_axes)
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        q_out = q.new_empty(q.shape)
     if k_out is None:
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    _check_heads(q_out, "q_out", q)
-    _check_heads(k_out, "k_out", k)
-    if q_out.shape != q.shape or k_out.shape != k.shape:
-        raise ValueError("q_out and k_out must match q and k")
-    _call(_dev_index(q), "mz_qk_norm_rope", q_out.data_ptr(), q_out.stride(0), q_out.stride(1),
-          k_out.data_ptr(), k_out.stride(0), k_out.stride(1), q.data_ptr(), q.stride(0),
-          q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), None, 0, 0, None, None, None, 0, 0,
-          *args, q.shape[0], q.shape[1], k.shape[1], q.shape[2], dtype_code(q.dtype))
+        k_out = k.new_empty(k.shape)
+    T, Hq, D = q.shape
+    Hkv = k.shape[1]
+    qo_at, ko_at = _heads(q_out, "q_out", q, Hq), _heads(k_out, "k_out", q, Hkv)
+    _call(_dev_index(q), "mz_qk_norm_rope", *qo_at, *ko_at, *q_at, *k_at, None, 0, 0, None, None, None, 0, 0, *args,
+          T, Hq, Hkv, D, dtype_code(q.dtype))
     return q_out, k_out
 
 
@@ -369,30 +390,22 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     to their slots of the pools.  slot_mapping: int64 ``[T]``, distinct; a
     negative slot skips the write."""
     n_blocks, H, bs, D = _check_pools(k_pool, v_pool)
-    if q.dim() != 3 or q.shape[2] != D or q.stride(2) != 1 or q.dtype != k_pool.dtype or \
-            q.device != k_pool.device:
-        raise ValueError(f"q must be [T, heads, {D}] of the pools' dtype and device with unit "
-                         "last stride")
-    _check_heads(k, "k", q)
-    _check_heads(v, "v", q)
-    if k.shape[1] != H or v.shape[1] != H:
-        raise ValueError(f"k and v must have the pools' {H} heads")
-    T = q.shape[0]
-    if slot_mapping.dtype != torch.int64 or slot_mapping.numel() != T or \
-            slot_mapping.device != q.device or not slot_mapping.is_contiguous():
+    if q.dim() != 3 or q.shape[2] != D or q.dtype is not k_pool.dtype or \
+            q.get_device() != k_pool.get_device():
+        raise ValueError(f"q must be [T, heads, {D}] of the pools' dtype and device")
+    q_at, k_at, v_at = _heads(q, "q", q), _heads(k, "k", q, H), _heads(v, "v", q, H)
+    T, Hq, _ = q.shape
+    if slot_mapping.dtype is not torch.int64 or slot_mapping.numel() != T or \
+            slot_mapping.get_device() != q.get_device() or not slot_mapping.is_contiguous():
         raise ValueError("slot_mapping must be a contiguous int64 [T] on the pool device")
-    args = _rope_args(q, k, positions, inv_freq, q_weight, k_weight, eps, weight_offset,
-                      interleaved, freq_axes)
+    args = _rope_args(q, positions, inv_freq, q_weight, k_weight, eps, weight_offset, interleaved,
+                      freq_axes)
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _check_heads(q_out, "q_out", q)
-    if q_out.shape != q.shape:
-        raise ValueError("q_out must match q")
-    _call(_dev_index(q), "mz_qk_norm_rope", q_out.data_ptr(), q_out.stride(0), q_out.stride(1),
-          None, 0, 0, q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0),
-          k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), k_pool.data_ptr(),
-          v_pool.data_ptr(), slot_mapping.data_ptr(), bs, n_blocks, *args, T, q.shape[1], H, D,
-          dtype_code(q.dtype))
+        q_out = q.new_empty(q.shape)
+    qo_at = _heads(q_out, "q_out", q, Hq)
+    _call(_dev_index(q), "mz_qk_norm_rope", *qo_at, None, 0, 0, *q_at, *k_at,
+          *v_at, k_pool.data_ptr(), v_pool.data_ptr(), slot_mapping.data_ptr(), bs, n_blocks,
+          *args, T, Hq, H, D, dtype_code(q.dtype))
     return q_out
 
 
@@ -407,6 +420,11 @@ def decode_workspace(n_seqs: int, n_kv_heads: int, rows: int, head_dim: int, dev
     kept for this layout (``shared``), or a new one the caller owns.  A
     batch-invariant launch needs room for the pieces of tables ``max_blocks``
     wide (of ``block_size``-token blocks)."""
+    key = (device, n_seqs, n_kv_heads, rows, head_dim, num_warps,
+           (max_blocks, block_size) if batch_invariant else None)
+    if shared and key in _workspaces:
+        _workspaces.move_to_end(key)
+        return _workspaces[key]
     size = ctypes.c_size_t(0)
     if batch_invariant:
         if max_blocks <= 0:
@@ -417,8 +435,6 @@ def decode_workspace(n_seqs: int, n_kv_heads: int, rows: int, head_dim: int, dev
     else:
         nat.call("mz_paged_decode_workspace_size", n_seqs, n_kv_heads, rows, head_dim,
                  num_warps, device, ctypes.byref(size))
-    key = (device, n_seqs, n_kv_heads, rows, head_dim, num_warps,
-           (max_blocks, block_size) if batch_invariant else None)
     return _layout_workspace(_workspaces, key, int(size.value), device, shared)
 
 
