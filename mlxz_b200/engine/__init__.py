@@ -3,6 +3,7 @@ the ragged continuous-batching decode step and chunked prefill."""
 from .decode_step import (PagedDecodeStep, PagedKVStore, QuantizedPagedDecodeStep,
                           QuantizedPagedKVStore)
 from .prefill import ChunkedPrefillScheduler, PagedPrefillStep, PrefillChunk
+from .qk_rope import QKNormRope
 
 __all__ = ["ChunkedPrefillScheduler", "PagedDecodeStep", "PagedKVStore", "PagedPrefillStep",
-           "PrefillChunk", "QuantizedPagedDecodeStep", "QuantizedPagedKVStore"]
+           "PrefillChunk", "QKNormRope", "QuantizedPagedDecodeStep", "QuantizedPagedKVStore"]

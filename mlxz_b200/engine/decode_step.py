@@ -20,6 +20,7 @@ import torch
 
 from .. import ops
 from ..paged_attention.block_manager import BlockManager
+from .qk_rope import QKNormRope, per_layer
 
 
 class PagedKVStore:
@@ -147,6 +148,10 @@ class PagedKVStore:
         return grew
 
 
+_NO_MOD = dict(softcap=0.0, alibi_slopes=None, window=0, sink_tokens=0, prefix_lens=None,
+               first_keys=None)
+
+
 def _copy_groups(n_layers: int) -> list[tuple[int, int]]:
     """[a, b) layer ranges with boundaries at 0, 1, 2, 4, ... from each end."""
     cuts, b = {0, n_layers}, 1
@@ -167,13 +172,28 @@ class PagedDecodeStep:
     them from (pinned) host memory and copies the output back.
     ``batch_invariant``: every sequence's output bytes are independent of the
     batch (each (sequence, KV head) pair is computed whole by one warp).
+
+    ``rope``: one QKNormRope or one per layer, applied to q and the new keys as
+    projected, at ``rope_positions`` (int32 ``[B]`` or ``[axes, B]``, which the
+    caller keeps up to date; default: the write positions).  ``softcap``,
+    ``alibi_slopes``, ``window``, ``sink_tokens``, ``prefix_lens`` and
+    ``first_keys`` as in ``ops.paged_decode``.
     """
 
     def __init__(self, store: PagedKVStore, seq_ids: list[str], n_heads: int,
                  scale: float | None = None, max_blocks: int | None = None,
-                 batch_invariant: bool = False) -> None:
+                 batch_invariant: bool = False,
+                 rope: "QKNormRope | list[QKNormRope] | None" = None,
+                 rope_positions: torch.Tensor | None = None, softcap: float = 0.0,
+                 alibi_slopes: torch.Tensor | None = None, window: int = 0, sink_tokens: int = 0,
+                 prefix_lens: torch.Tensor | None = None,
+                 first_keys: torch.Tensor | None = None) -> None:
         self.store = store
         self.batch_invariant = batch_invariant
+        self.rope = per_layer(rope, store.n_layers)
+        self._rope_positions = rope_positions
+        self._mod = dict(softcap=softcap, alibi_slopes=alibi_slopes, window=window,
+                         sink_tokens=sink_tokens, prefix_lens=prefix_lens, first_keys=first_keys)
         self.seq_ids = list(seq_ids)
         self.n_heads = n_heads
         self.scale = scale if scale is not None else store.head_dim ** -0.5
@@ -211,6 +231,28 @@ class PagedDecodeStep:
         self.tables.copy_(host, non_blocking=False)
         self.positions.copy_(offs)
         self.lengths.copy_(offs + 1)
+        # blocks of each table that the device has
+        self._uploaded = [len(self.store.tables[s]) for s in self.seq_ids]
+        self._held = torch.tensor(self._uploaded, dtype=torch.int32).to(self.store.device)
+
+    @property
+    def plain(self) -> bool:
+        """No rope and no modified scores or masks."""
+        return self._mod_off() and all(r is None for r in self.rope)
+
+    def _mod_off(self) -> bool:
+        m = self._mod
+        return not (m["softcap"] or m["window"]) and all(
+            m[k] is None for k in ("alibi_slopes", "prefix_lens", "first_keys"))
+
+    def _turn(self, l: int, q: torch.Tensor, k_new: torch.Tensor
+              ) -> tuple[torch.Tensor, torch.Tensor]:
+        """Layer l's norm and rotation of q and the new keys."""
+        rope = self.rope[l]
+        if rope is None:
+            return q, k_new
+        pos = self.positions if self._rope_positions is None else self._rope_positions
+        return rope.apply(q, k_new, pos)
 
     def layer(self, l: int, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
               out: torch.Tensor, num_warps: int = 0) -> None:
@@ -219,10 +261,12 @@ class PagedDecodeStep:
         launch finishes (it writes none of this layer's pools, and the tables
         and lengths change only between steps)."""
         st = self.store
+        q, k_new = self._turn(l, q, k_new)
         ops.paged_append_decode(q, st.k_pool(l), st.v_pool(l), k_new, v_new, self.tables,
                                 self.lengths, scale=self.scale, out=out,
                                 workspace=self.workspace, num_warps=num_warps,
-                                overlap_previous=l > 0, batch_invariant=self.batch_invariant)
+                                overlap_previous=l > 0, batch_invariant=self.batch_invariant,
+                                **self._mod)
 
     def prepare_writes(self) -> int:
         """Copy-on-write every block this step will write that is shared (a
@@ -251,16 +295,32 @@ class PagedDecodeStep:
         return out
 
     def advance(self) -> None:
-        """Commit the appended token: offsets += 1, growing tables as needed."""
-        grew = False
-        for s in self.seq_ids:
-            self.store.offsets[s] += 1
-            grew |= self.store.ensure_capacity(s, 1)
-        if grew:
+        """Commit the appended token: offsets += 1, growing tables as needed.
+        New blocks' ids go up alone; mz_paged_plan puts them into the tables."""
+        st = self.store
+        new: list[int] = []
+        in_step = True  # the device's tables are what the host's were before
+        for i, s in enumerate(self.seq_ids):
+            st.offsets[s] += 1
+            had = len(st.tables[s])
+            st.ensure_capacity(s, 1)
+            new += st.tables[s][had:]
+            in_step &= had == self._uploaded[i] and len(st.tables[s]) <= self.max_blocks
+        if new and not in_step:
             self.sync_metadata()
-        else:
-            self.positions.add_(1)
-            self.lengths.add_(1)
+            return
+        self.positions.add_(1)
+        self.lengths.add_(1)
+        if new:
+            if self._ones is None:
+                self._ones = torch.ones_like(self.positions)
+            ids = torch.tensor(new, dtype=torch.int32).to(st.device, non_blocking=True)
+            plan = ops.paged_plan(self.tables, self.positions, self._ones, self.B, st.block_size,
+                                  st.n_blocks, new_ids=ids, held=self._held)
+            self._held = plan.held
+            self._uploaded = [len(st.tables[s]) for s in self.seq_ids]
+
+    _ones: torch.Tensor | None = None
 
     def capture(self, q_dtype: torch.dtype | None = None) -> None:
         """Capture every layer's launch of one step into a CUDA graph over
@@ -421,11 +481,17 @@ class QuantizedPagedKVStore(PagedKVStore):
 class QuantizedPagedDecodeStep(PagedDecodeStep):
     """Decode step over a QuantizedPagedKVStore: per layer, quantise-on-append
     of the new token (mz_kv_quant_append_paged), then attention with the
-    dequantisation fused in (mz_paged_decode_q)."""
+    dequantisation fused in (mz_paged_decode_q).  ``rope`` as in PagedDecodeStep;
+    the quantised decode has no modified scores or masks."""
 
     def __init__(self, store: QuantizedPagedKVStore, seq_ids: list[str], n_heads: int,
-                 scale: float | None = None, max_blocks: int | None = None) -> None:
+                 scale: float | None = None, max_blocks: int | None = None,
+                 rope: "QKNormRope | list[QKNormRope] | None" = None,
+                 rope_positions: torch.Tensor | None = None) -> None:
         self.store = store
+        self.rope = per_layer(rope, store.n_layers)
+        self._rope_positions = rope_positions
+        self._mod = _NO_MOD
         self.seq_ids = list(seq_ids)
         self.n_heads = n_heads
         self.scale = scale if scale is not None else store.head_dim ** -0.5
@@ -450,6 +516,7 @@ class QuantizedPagedDecodeStep(PagedDecodeStep):
     def layer(self, l: int, q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor,
               out: torch.Tensor, num_warps: int = 0) -> None:
         pools = self.store.qpools(l)
+        q, k_new = self._turn(l, q, k_new)
         ops.kv_quant_append_paged(pools, k_new, v_new, self.tables, self.positions)
         ops.paged_decode_q(q, pools, self.tables, self.lengths, scale=self.scale, out=out,
                            workspace=self.workspace, num_warps=num_warps)

@@ -16,6 +16,12 @@ Queries and new K/V arrive as the model's projections lay them out: q
 ``[T, Hq, D]`` and k / v ``[T, Hkv, D]``, the sequences' chunks stacked along
 T in the order given.
 
+The slots, positions and lengths of a step come from one mz_paged_plan launch.
+With ``rope`` the queries and keys arrive as projected: their norm, rotation and
+append are one mz_qk_norm_rope launch per layer in place of mz_kv_append.  With
+a soft cap, slopes, a window, prefix or document masks the attention is
+mz_paged_prefill_mod.
+
 Over a QuantizedPagedKVStore the chunk is quantised on append
 (mz_kv_quant_append) and the chunk attends over the quantised keys and values,
 as a quantised cache's attention does: per layer the step's blocks are
@@ -30,6 +36,7 @@ import torch
 
 from .. import ops
 from .decode_step import PagedKVStore, QuantizedPagedKVStore
+from .qk_rope import QKNormRope, per_layer
 
 
 @dataclass(slots=True)
@@ -81,10 +88,21 @@ class PagedPrefillStep:
     at each sequence's current offset.  Construction grows the block tables
     (copy-on-write of a shared block at the offset) and uploads the step's
     tables, slots and lengths once; ``layer`` runs append + attention for one
-    layer; ``finish`` advances the sequences' offsets."""
+    layer; ``finish`` advances the sequences' offsets.
+
+    ``rope``: one QKNormRope or one per layer, applied to q and k at
+    ``rope_positions`` (int32 ``[T]`` or ``[axes, T]``; default: each token's
+    position in its sequence).  ``softcap``, ``alibi_slopes``, ``window``,
+    ``sink_tokens`` and ``first_keys`` (int32 ``[T]``) as in
+    ``ops.paged_prefill``; ``prefix_lens``: one number per chunk."""
 
     def __init__(self, store: PagedKVStore, chunks: list[tuple[str, int]], n_heads: int,
-                 scale: float | None = None) -> None:
+                 scale: float | None = None,
+                 rope: "QKNormRope | list[QKNormRope] | None" = None,
+                 rope_positions: torch.Tensor | None = None, softcap: float = 0.0,
+                 alibi_slopes: torch.Tensor | None = None, window: int = 0, sink_tokens: int = 0,
+                 prefix_lens: list[int] | None = None,
+                 first_keys: torch.Tensor | None = None) -> None:
         if not isinstance(store, PagedKVStore):
             raise TypeError("chunked prefill needs a PagedKVStore")
         self.quantized = isinstance(store, QuantizedPagedKVStore)
@@ -94,7 +112,9 @@ class PagedPrefillStep:
         self.chunks = [(s, int(n)) for s, n in chunks]
         self.n_heads = n_heads
         self.scale = scale if scale is not None else store.head_dim ** -0.5
-        bs = store.block_size
+        self.rope = per_layer(rope, store.n_layers)
+        if prefix_lens is not None and len(prefix_lens) != len(self.chunks):
+            raise ValueError("prefix_lens must hold one number per chunk")
         cow = []
         for s, n in self.chunks:
             store.ensure_capacity(s, n)
@@ -107,30 +127,33 @@ class PagedPrefillStep:
         self.T = sum(n for _, n in self.chunks)
         width = max([1] + [len(store.tables[s]) for s, _ in self.chunks])
         tables = torch.full((B, width), -1, dtype=torch.int32)
+        lens = torch.zeros((3, B), dtype=torch.int32)  # cached, new, blocks in the table
+        for b, (s, n) in enumerate(self.chunks):
+            t = store.tables[s]
+            tables[b, :len(t)] = torch.tensor(t, dtype=torch.int32)
+            lens[0, b], lens[1, b], lens[2, b] = store.offsets[s], n, len(t)
+        dev = store.device
+        self.max_q_len = max([0] + [n for _, n in self.chunks])
+        self.tables = tables.to(dev)
+        cached, self.q_len, held = lens.to(dev)
+        plan = ops.paged_plan(self.tables, cached, self.q_len, self.T, store.block_size,
+                              store.n_blocks, held=held)
+        self.q_start, self.ctx_lens, self.slots = plan.q_start, plan.lengths, plan.slots
+        self.positions = plan.positions
+        self.rope_positions = self.positions if rope_positions is None else rope_positions
+        self._mod = dict(softcap=softcap, alibi_slopes=alibi_slopes, window=window,
+                         sink_tokens=sink_tokens, first_keys=first_keys,
+                         prefix_lens=None if prefix_lens is None else
+                         torch.tensor(prefix_lens, dtype=torch.int32).to(dev))
         # quantised store: the attention reads a staging pool holding the
         # step's blocks in first-use order, through renumbered tables
         uniq = list(dict.fromkeys(blk for s, _ in self.chunks for blk in store.tables[s]))
-        local = {blk: i for i, blk in enumerate(uniq)}
-        q_start, q_len, ctx, slots = [], [], [], []
-        row = 0
-        for b, (s, n) in enumerate(self.chunks):
-            t = store.tables[s]
-            tt = [local[blk] for blk in t] if self.quantized else t
-            if tt:
-                tables[b, :len(tt)] = torch.tensor(tt, dtype=torch.int32)
-            off = store.offsets[s]
-            q_start.append(row)
-            q_len.append(n)
-            ctx.append(off + n)
-            slots.extend(t[p // bs] * bs + p % bs for p in range(off, off + n))
-            row += n
-        dev = store.device
-        self.max_q_len = max([0] + q_len)
-        self.tables = tables.to(dev)
-        self.q_start = torch.tensor(q_start, dtype=torch.int32).to(dev)
-        self.q_len = torch.tensor(q_len, dtype=torch.int32).to(dev)
-        self.ctx_lens = torch.tensor(ctx, dtype=torch.int32).to(dev)
-        self.slots = torch.tensor(slots, dtype=torch.int64).to(dev)
+        if self.quantized:
+            local = {blk: i for i, blk in enumerate(uniq)}
+            for b, (s, _) in enumerate(self.chunks):
+                t = store.tables[s]
+                tables[b, :len(t)] = torch.tensor([local[blk] for blk in t], dtype=torch.int32)
+            self.tables = tables.to(dev)
         self._ids = torch.tensor(uniq, dtype=torch.int32).to(dev) if self.quantized else None
         self._stage = None
         self._done = False
@@ -145,8 +168,11 @@ class PagedPrefillStep:
             raise ValueError(f"k/v must be [{self.T}, {st.n_kv_heads}, {st.head_dim}]")
         if q.shape != (self.T, self.n_heads, st.head_dim):
             raise ValueError(f"q must be [{self.T}, {self.n_heads}, {st.head_dim}]")
+        rope = self.rope[l]
         if self.quantized:
             pools = st.qpools(l)
+            if rope is not None and self.T:
+                q, k = rope.apply(q, k, self.rope_positions)
             ops.kv_quant_append(pools, k.transpose(0, 1), v.transpose(0, 1), self.slots)
             shape = (self._ids.numel(), st.n_kv_heads, st.block_size, st.head_dim)
             if self._stage is None or self._stage[0].dtype != q.dtype:
@@ -156,9 +182,13 @@ class PagedPrefillStep:
             ops.kv_dequant_blocks(pools, self._ids, kp, vp)
         else:
             kp, vp = st.k_pool(l), st.v_pool(l)
-            ops.kv_append(kp, vp, k.transpose(0, 1), v.transpose(0, 1), self.slots)
+            if rope is not None:
+                q = rope.apply_append(q, k, v, self.rope_positions, kp, vp, self.slots)
+            else:
+                ops.kv_append(kp, vp, k.transpose(0, 1), v.transpose(0, 1), self.slots)
         return ops.paged_prefill(q, kp, vp, self.tables, self.q_start, self.q_len, self.ctx_lens,
-                                 self.max_q_len, self.scale, out=out, out_dtype=out_dtype)
+                                 self.max_q_len, self.scale, out=out, out_dtype=out_dtype,
+                                 **self._mod)
 
     def finish(self) -> None:
         """Advance every sequence's offset past its chunk (once all layers ran)."""

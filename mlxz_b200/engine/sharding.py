@@ -247,6 +247,9 @@ class PeerAllGather:
         that launch's slot for work queued after this one."""
         from .. import ops
 
+        if not getattr(step, "plain", True):
+            raise ValueError("the fused all-gather runs plain decode steps: without rope, "
+                             "modified scores or masks")
         self._check_slot(slot, wait_previous)
         self.epoch = self.epoch % 0xFFFFFFFF + 1  # 1, 2, ..., 2^32 - 1, 1, ...
         pe = self._peers[slot]

@@ -415,13 +415,15 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 
 def decode_workspace(n_seqs: int, n_kv_heads: int, rows: int, head_dim: int, device: int,
                      num_warps: int = 0, shared: bool = True, batch_invariant: bool = False,
-                     max_blocks: int = 0, block_size: int = 16) -> torch.Tensor:
+                     max_blocks: int = 0, block_size: int = 16,
+                     stream: int | None = None) -> torch.Tensor:
     """A zero-initialised decode workspace for exactly these sizes: the one
-    kept for this layout (``shared``), or a new one the caller owns.  A
+    kept for this layout (``shared``; with ``stream``, a stream's raw handle,
+    for this layout on that stream), or a new one the caller owns.  A
     batch-invariant launch needs room for the pieces of tables ``max_blocks``
     wide (of ``block_size``-token blocks)."""
     key = (device, n_seqs, n_kv_heads, rows, head_dim, num_warps,
-           (max_blocks, block_size) if batch_invariant else None)
+           (max_blocks, block_size) if batch_invariant else None, stream)
     if shared and key in _workspaces:
         _workspaces.move_to_end(key)
         return _workspaces[key]
@@ -463,6 +465,19 @@ def _score_mod(n_heads: int, device: torch.device, softcap: float,
     big = (1 << 31) - 1
     return nat.ScoreMod(softcap, min(window, big), min(sink_tokens, big), _ptr(alibi_slopes),
                         _ptr(prefix_lens), _ptr(first_keys))
+
+
+def _mod_workspace(n_seqs: int, n_kv_heads: int, rows: int, head_dim: int, device: int,
+                   num_warps: int, **kw) -> torch.Tensor:
+    """The workspace of a modified-score call that was given none: one per
+    layout and stream, so that calls on two streams do not meet in it, and a
+    new one inside a capture (its clearing is captured with it), so that no
+    two graphs do."""
+    if torch.cuda.is_current_stream_capturing():
+        return decode_workspace(n_seqs, n_kv_heads, rows, head_dim, device, num_warps,
+                                shared=False, **kw)
+    return decode_workspace(n_seqs, n_kv_heads, rows, head_dim, device, num_warps,
+                            stream=_stream(device), **kw)
 
 
 def reset_workspaces() -> None:
@@ -535,7 +550,8 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     dev = _dev_index(q)
     rows = nq * (Hq // Hkv)
     if workspace is None:
-        workspace = decode_workspace(B, Hkv, rows, D, dev, num_warps)
+        workspace = (decode_workspace if mod is None else _mod_workspace)(B, Hkv, rows, D, dev,
+                                                                          num_warps)
     if mod is not None:
         _call(dev, "mz_paged_decode_mod", out.data_ptr(), dtype_code(out_dtype), o_sb, o_st, o_sh,
               q.data_ptr(), q_sb, q_st, q_sh, nq, k_pool.data_ptr(), v_pool.data_ptr(),
@@ -596,9 +612,9 @@ def paged_append_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Ten
         return out
     dev = _dev_index(q)
     if workspace is None:
-        workspace = decode_workspace(B, Hkv, Hq // Hkv, D, dev, num_warps,
-                                     batch_invariant=batch_invariant,
-                                     max_blocks=block_tables.shape[1], block_size=bs)
+        workspace = (decode_workspace if mod is None else _mod_workspace)(
+            B, Hkv, Hq // Hkv, D, dev, num_warps, batch_invariant=batch_invariant,
+            max_blocks=block_tables.shape[1], block_size=bs)
     if mod is not None:
         _call(dev, "mz_paged_append_decode_mod", out.data_ptr(), dtype_code(out_dtype),
               out.stride(0), out.stride(1), q.data_ptr(), q.stride(0), q.stride(1),

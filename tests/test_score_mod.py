@@ -448,3 +448,34 @@ def test_oracle_masks():
     v = osm.visible(np.array([1, 5]), 8, window=2, prefix=3, first=np.array([0, 5]))
     assert v[0].tolist() == [True] * 3 + [False] * 5
     assert v[1].tolist() == [True] * 3 + [False] * 2 + [True] + [False] * 2
+
+
+@gpu
+def test_default_workspaces_of_two_streams_and_of_two_graphs(cuda):
+    """Calls that bring no workspace, at once on two streams, and two captured
+    graphs replayed at once."""
+    dtype, D, G, ctx = "bf16", 128, 4, [3000, 70, 900]
+    case = random_paged_case(33, 3, 2, D, 16, ctx, dtype, G=G)
+    kp, vp, tables, c = _dev(case, dtype, cuda)
+    q = to_dev(case["q"][:, 0], dtype, cuda)
+    kw = dict(window=2000, sink_tokens=4, softcap=30.0)
+    want = osm.paged(case["q"][:, 0], case["kp"], case["vp"], case["tables"], np.arange(3),
+                     np.ones(3, dtype=int), case["ctx"], dtype, softcap=30.0, window=2000, sink=4)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    graphs, outs = [], []
+    torch.cuda.synchronize()
+    for s in streams:
+        with torch.cuda.stream(s):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                outs.append(ops.paged_decode(q, kp, vp, tables, c, **kw))
+            graphs.append(g)
+    for _ in range(20):
+        for s, g in zip(streams, graphs):
+            with torch.cuda.stream(s):
+                outs.append(ops.paged_decode(q, kp, vp, tables, c, **kw))
+                g.replay()
+    torch.cuda.synchronize()
+    ops.check_device_errors(0)
+    for o in outs:
+        _check(o, want)
