@@ -203,6 +203,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) give_up();
     return false;
   };
+  // two barriers that are mostly both there: one round trip for the two polls
+  auto wait2 = [&](int b0, int phase0, int b1, int phase1) {
+    const bool x = mbar_try_wait(bar(b0), phase0 & 1), y = mbar_try_wait(bar(b1), phase1 & 1);
+    if (__all_sync(0xffffffffu, x && y)) return true;
+    return wait(b0, phase0) && wait(b1, phase1);
+  };
 
   Item it;
   int g = 0;  // tiles of this stream so far: slot g % 2, barrier phase g / 2
@@ -293,8 +299,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto issue_s = [&](int j) -> bool {
       const int s = j & 1;
       // K is there; the buffer is free once the P.V that read its P is computed
-      if (!wait(kBarKFull + s, j >> 1)) return false;
-      if (j >= kSlots && !wait(kBarPvDone + s, (j - kSlots) >> 1)) return false;
+      if (j < kSlots ? !wait(kBarKFull + s, 0)
+                     : !wait2(kBarPvDone + s, (j - kSlots) >> 1, kBarKFull + s, j >> 1))
+        return false;
       tc::fence_after_sync();
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
@@ -318,7 +325,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const int j = g + i, s = j & 1;
         // P of an item's first tile is written after the item before's O is read
-        if (!wait(kBarPFull + s, j >> 1) || !wait(kBarVFull + s, j >> 1)) {
+        if (!wait2(kBarPFull + s, j >> 1, kBarVFull + s, j >> 1)) {
           ok = false;
           break;
         }
