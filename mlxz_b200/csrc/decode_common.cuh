@@ -157,7 +157,6 @@ __device__ __forceinline__ int span_tiles(const ModParams &p, int b, int ctx) {
 }
 
 // The sequence's own tile that a cursor's tile t stands for.
-__device__ __forceinline__ int own_tile(const Params &, int, int t, int, int) { return t; }
 __device__ __forceinline__ int own_tile(const ModParams &p, int b, int t, int n, int ctx) {
   const int skip = ntiles_of(ctx) - n;
   if (skip == 0) return t;
@@ -867,6 +866,11 @@ inline void set_schedule(Params &p, const WsLayout &ws) {
   p.static_pct = env_int("MLXZ_B200_DECODE_STATIC_PCT", 100, 1, 100);
   p.min_chunk = env_int("MLXZ_B200_DECODE_MIN_CHUNK", 16, 1, 1 << 20);
 }
+
+// The launch of a decode with modified scores and masks (paged_decode_mod.cu);
+// cfg has grid, block, stream and attributes.
+int launch_mod(cudaLaunchConfig_t &cfg, int D, bool bf16, const CUtensorMap &tk,
+               const CUtensorMap &tv, const ModParams &p, const char *fn);
 
 // Occupancy of a decode kernel instantiation (cached; also sets its shared
 // memory attribute once).

@@ -22,8 +22,6 @@
 // us static, 237 us with 15 % in 9-tile chunks: every chunk adds a piece to
 // merge), so the default hands out everything statically; merges of split
 // pairs are deferred to the end of each warp's loop.
-#include <type_traits>
-
 #include "decode_common.cuh"
 
 #ifndef MZ_DECODE_STAGES_D128
@@ -45,11 +43,9 @@ struct Cfg {
   static constexpr int kSmemBytes = kSmemTiles + kSmemBars + kSmemUnits + kSmemDefer + 1024;
 };
 
-// P: Params, or ModParams for modified scores and masks.
-template <int D, bool BF16, bool GATHER, class P>
+template <int D, bool BF16, bool GATHER>
 __device__ __forceinline__ void decode_tiles(const CUtensorMap &tmK, const CUtensorMap &tmV,
-                                             const P &p) {
-  constexpr bool MOD = std::is_same<P, ModParams>::value;
+                                             const Params &p) {
   using C = Cfg<D>;
   constexpr int S = C::kStages;
   constexpr int KS = D / 16;  // k-steps of Q.K^T, also n-tile pairs of P.V
@@ -84,13 +80,12 @@ __device__ __forceinline__ void decode_tiles(const CUtensorMap &tmK, const CUten
   const uint64_t pol = l2_policy_evict_first();
   auto issue = [&](int s, const Cursor &c) {
     if (lane == 0) {
-      const int t = own_tile(p, c.b, c.t, c.n, c.ctx);
-      int32_t blk = p.tables[(int64_t)c.b * p.max_blocks + t / p.tpb];
+      int32_t blk = p.tables[(int64_t)c.b * p.max_blocks + c.t / p.tpb];
       if (blk < 0 || blk >= p.n_blocks) {
         dev_error(p.err, MZ_DEVERR_BLOCK_ID);
         blk = 0;
       }
-      const int y = static_cast<int>(((int64_t)blk * p.Hkv + c.h) * p.bs + (t % p.tpb) * kTileTok);
+      const int y = static_cast<int>(((int64_t)blk * p.Hkv + c.h) * p.bs + (c.t % p.tpb) * kTileTok);
       const uint32_t bar = bar0 + 8 * s;
       const uint32_t dk = stage0 + s * C::kStageBytes;
       mbar_arrive_expect_tx(bar, C::kStageBytes);
@@ -115,10 +110,6 @@ __device__ __forceinline__ void decode_tiles(const CUtensorMap &tmK, const CUten
 
   UnitReader ur;
   bool seg_first = true;
-  // MOD: the piece's mask, and the positions, lower ends and slopes of rows g, g + 8
-  MaskSpan span{};
-  int skip = 0, p_min = 0, lo_max = 0, pos0 = 0, pos1 = 0, lo0 = 0, lo1 = 0;
-  float slope0 = 0.f, slope1 = 0.f;
 
   // Until the launch ahead has completed (programmatic dependent launch) only
   // ctx, the tables and the pools are read: the first tiles of the static
@@ -142,25 +133,8 @@ __device__ __forceinline__ void decode_tiles(const CUtensorMap &tmK, const CUten
     if (seg_first || cc.t == 0) {
       // New piece: load the grouped query rows as A fragments.
       seg_first = false;
-      m0 = m1 = MOD ? kNoMax : -INFINITY;
+      m0 = m1 = -INFINITY;
       l0 = l1 = 0.f;
-      if constexpr (MOD) {
-        span = mask_span(p, cc.b, cc.ctx);
-        skip = ntiles_of(cc.ctx) - cc.n;
-        p_min = cc.ctx - p.n_q;
-        pos0 = p_min + g / p.G;
-        pos1 = p_min + (g + 8) / p.G;
-        // lower ends rise with the token where the window sets them
-        const int first = p.mod.first ? max(0, p.mod.first[cc.b]) : 0;
-        const int w = p.mod.window > 0 ? p.mod.window : 1 << 30;
-        lo0 = max(first, pos0 - w + 1);
-        lo1 = max(first, pos1 - w + 1);
-        lo_max = max(first, cc.ctx - w);
-        if (p.mod.slopes) {
-          slope0 = g < p.rows ? p.mod.slopes[cc.h * p.G + g % p.G] * kLog2e : 0.f;
-          slope1 = g + 8 < p.rows ? p.mod.slopes[cc.h * p.G + (g + 8) % p.G] * kLog2e : 0.f;
-        }
-      }
 #pragma unroll
       for (int n = 0; n < NT; ++n) oacc[n][0] = oacc[n][1] = oacc[n][2] = oacc[n][3] = 0.f;
       const auto *q16 = static_cast<const uint16_t *>(p.q);
@@ -186,9 +160,7 @@ __device__ __forceinline__ void decode_tiles(const CUtensorMap &tmK, const CUten
     uint8_t *vt = kt + C::kTileBytes;
     const uint32_t kb = stage0 + s * C::kStageBytes;
     const uint32_t vb = kb + C::kTileBytes;
-    const int tile = MOD && cc.t >= ntiles_of(span.head) ? cc.t + skip : cc.t;  // own_tile
-    const int key0 = tile * kTileTok;
-    const int nvalid = min(kTileTok, cc.ctx - key0);
+    const int nvalid = min(kTileTok, cc.ctx - cc.t * kTileTok);
     const bool last_tile = (cc.t == cc.n - 1);
     if (p.kn != nullptr && last_tile) {
       // Fused append: the sequence's new token is its last attended one.  Write
@@ -212,15 +184,7 @@ __device__ __forceinline__ void decode_tiles(const CUtensorMap &tmK, const CUten
       }
       __syncwarp();
     }
-    if (MOD && key0 < span.lo && key0 + kTileTok > span.head) {
-      // Keys that no row sees may hold anything: exact zeros for V here too.
-      for (int e = lane; e < kTileTok * (D / 8); e += 32) {
-        const int tok = e / (D / 8), d = (e % (D / 8)) * 8, key = key0 + tok;
-        if (key >= cc.ctx || (key < span.lo && key >= span.head))
-          *reinterpret_cast<uint4 *>(vt + swz128(tok, 2 * d)) = make_uint4(0, 0, 0, 0);
-      }
-      __syncwarp();
-    } else if (nvalid < kTileTok) {
+    if (nvalid < kTileTok) {
       // Rows past the context may hold stale data; make them exact zeros so
       // that 0 * V stays 0 in P.V.
       for (int e = lane; e < (kTileTok - nvalid) * (D / 8); e += 32) {
@@ -244,59 +208,16 @@ __device__ __forceinline__ void decode_tiles(const CUtensorMap &tmK, const CUten
 
     // Online softmax (exp2 domain), rows g (regs 0,1) and g+8 (regs 2,3).
     float mx0 = -INFINITY, mx1 = -INFINITY;
-    if constexpr (MOD) {
-      // rows g + 8 only where there are any
-      const int ne = two_groups ? 4 : 2;
-      if (p.mod.z_scale == 0.f) {
 #pragma unroll
-        for (int x = 0; x < 8; ++x)
-          if ((x & 3) < ne) sacc[x >> 2][x & 3] *= p.scale_log2;
-      } else if (p.mod.cap_log2 <= kQuickCapLog2) {
+    for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int x = 0; x < 8; ++x)
-          if ((x & 3) < ne) sacc[x >> 2][x & 3] = cap_quick(p.mod, sacc[x >> 2][x & 3]);
-      } else {
-#pragma unroll
-        for (int x = 0; x < 8; ++x)
-          if ((x & 3) < ne)
-            sacc[x >> 2][x & 3] =
-                p.mod.cap_log2 * tanh_mod(sacc[x >> 2][x & 3] * p.mod.z_scale);
+      for (int e = 0; e < 4; ++e) {
+        const int tok = n * 8 + 2 * cq + (e & 1);
+        float x = sacc[n][e] * p.scale_log2;
+        if (tok >= nvalid) x = -INFINITY;
+        sacc[n][e] = x;
+        if (e < 2) mx0 = fmaxf(mx0, x); else mx1 = fmaxf(mx1, x);
       }
-      if (p.mod.slopes) {
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const int key = key0 + (x >> 2) * 8 + 2 * cq + (x & 1);
-          const float far = static_cast<float>(((x & 2) ? pos1 : pos0) - key);
-          sacc[x >> 2][x & 3] = fmaf(-((x & 2) ? slope1 : slope0), fabsf(far), sacc[x >> 2][x & 3]);
-        }
-      }
-      // not every row sees every key of the tile
-      if (!((key0 >= lo_max && key0 + kTileTok - 1 <= p_min) || key0 + kTileTok <= span.prefix)) {
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const int key = key0 + (x >> 2) * 8 + 2 * cq + (x & 1);
-          const int pos = (x & 2) ? pos1 : pos0, lo = (x & 2) ? lo1 : lo0;
-          if (!(key < span.prefix || (key <= pos && (key >= lo || key < p.mod.sink))))
-            sacc[x >> 2][x & 3] = -INFINITY;
-        }
-      }
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        mx0 = fmaxf(mx0, fmaxf(sacc[n][0], sacc[n][1]));
-        mx1 = fmaxf(mx1, fmaxf(sacc[n][2], sacc[n][3]));
-      }
-    } else {
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int tok = n * 8 + 2 * cq + (e & 1);
-          float x = sacc[n][e] * p.scale_log2;
-          if (tok >= nvalid) x = -INFINITY;
-          sacc[n][e] = x;
-          if (e < 2) mx0 = fmaxf(mx0, x); else mx1 = fmaxf(mx1, x);
-        }
-    }
     mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 1));
     mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
     const float mn0 = fmaxf(m0, mx0);
@@ -383,8 +304,7 @@ __device__ __forceinline__ void decode_tiles(const CUtensorMap &tmK, const CUten
       const int uf = p.batch_invariant ? sch.W + ur.fp : sch.unit_of(pbh);
       const int ul = p.batch_invariant ? uf + ur.np - 1 : sch.unit_of(pbh + cc.n - 1);
       if (uf == ul) {
-        const float i0 = MOD ? row_inverse(L0) : 1.f / L0;
-        const float i1 = !two_groups ? 0.f : MOD ? row_inverse(L1) : 1.f / L1;
+        const float i0 = 1.f / L0, i1 = two_groups ? 1.f / L1 : 0.f;
         if (g < p.rows) {
           const int64_t o = row_offset(p.o_sb, p.o_st, p.o_sh, cc.b, cc.h, g, p.G);
 #pragma unroll
@@ -437,15 +357,6 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
   decode_tiles<D, BF16, false>(tmK, tmV, p);
 }
 
-// Modified scores and masks (score_mod.cuh).
-template <int D, bool BF16>
-__global__ void __launch_bounds__(kWarps * 32, 2)
-    paged_decode_mod_kernel(const __grid_constant__ CUtensorMap tmK,
-                            const __grid_constant__ CUtensorMap tmV, const ModParams p) {
-  launch_dependents();
-  decode_tiles<D, BF16, false>(tmK, tmV, p);
-}
-
 // The all-gather instantiation: every output store also goes to the peers'
 // buffers, and the grid's last block signals them.
 template <int D, bool BF16>
@@ -481,13 +392,6 @@ int gather_smem_attr() {
   static DeviceOnce once;
   return smem_optin(paged_decode_gather_kernel<D, BF16>, Cfg<D>::kSmemBytes, once,
                     "setting the all-gather kernel's shared memory");
-}
-
-template <int D, bool BF16>
-int mod_smem_attr() {
-  static DeviceOnce once;
-  return smem_optin(paged_decode_mod_kernel<D, BF16>, Cfg<D>::kSmemBytes, once,
-                    "setting the modified-score kernel's shared memory");
 }
 
 int ctas_per_sm(int D, bool bf16, int *out) {
@@ -704,14 +608,12 @@ int launch(const DecodeArgs &a, int64_t warps, const WsLayout &ws, void *scratch
   attr[0].val.programmaticStreamSerializationAllowed = (a.flags & MZ_LAUNCH_OVERLAP_PREVIOUS) ? 1 : 0;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
+  if (a.mod) return launch_mod(cfg, a.D, bf16, tk, tv, mp, fn);
   cudaError_t le = cudaSuccess;
 #define MZ_LAUNCH(D_, BF_)                                                          \
   do {                                                                              \
     cfg.dynamicSmemBytes = Cfg<D_>::kSmemBytes;                                     \
-    if (a.mod) {                                                                    \
-      if (int rc = mod_smem_attr<D_, BF_>()) return rc;                             \
-      le = cudaLaunchKernelEx(&cfg, paged_decode_mod_kernel<D_, BF_>, tk, tv, mp);  \
-    } else if (a.peers) {                                                           \
+    if (a.peers) {                                                                  \
       if (int rc = gather_smem_attr<D_, BF_>()) return rc;                          \
       le = cudaLaunchKernelEx(&cfg, paged_decode_gather_kernel<D_, BF_>, tk, tv, p); \
     } else {                                                                        \
