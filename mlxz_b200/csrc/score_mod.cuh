@@ -67,8 +67,13 @@ constexpr float kQuickCapLog2 = 1000.f * kLog2e;
 inline int make_score_mod(ScoreMod *m, const mz_score_mod *mod, float scale, int64_t tokens,
                           const char *fn) {
   if (!mod) return fail(MZ_ERR_INVALID_ARG, "%s: mod is null", fn);
-  if (!std::isfinite(mod->softcap) || mod->softcap < 0.f)
-    return fail(MZ_ERR_INVALID_ARG, "%s: softcap must be finite and not negative", fn);
+  if (!std::isfinite(mod->softcap) || mod->softcap < 0.f ||
+      (mod->softcap > 0.f && !std::isfinite(scale / mod->softcap)))
+    return fail(MZ_ERR_INVALID_ARG,
+                "%s: softcap must be finite, not negative and not so small that scale / softcap "
+                "overflows", fn);
+  if (tokens >= (int64_t(1) << 31) - 1024)
+    return fail(MZ_ERR_UNSUPPORTED, "%s: tables span 2^31 or more tokens", fn);
   if (mod->window < 0 || mod->sink_tokens < 0)
     return fail(MZ_ERR_INVALID_ARG, "%s: window and sink_tokens must not be negative", fn);
   const void *ptrs[] = {mod->alibi_slopes, mod->prefix_lens, mod->first_keys};
@@ -80,19 +85,22 @@ inline int make_score_mod(ScoreMod *m, const mz_score_mod *mod, float scale, int
   // a window of the whole table hides nothing; no position exceeds it either
   m->window = mod->window >= tokens ? 0 : mod->window;
   m->sink = static_cast<int>(mod->sink_tokens < tokens ? mod->sink_tokens : tokens);
-  m->z_scale = mod->softcap > 0.f ? scale / mod->softcap : 0.f;
-  const double cap_log2 = static_cast<double>(mod->softcap) * 1.4426950408889634;
+  // a cap of 10^30 leaves every fp32 score as it is; scale / cap would near the
+  // smallest fp32 numbers there
+  const float cap = mod->softcap < 1e30f ? mod->softcap : 0.f;
+  m->z_scale = cap > 0.f ? scale / cap : 0.f;
+  const double cap_log2 = static_cast<double>(cap) * 1.4426950408889634;
   m->cap_log2 = static_cast<float>(cap_log2);
   // tanh(z) / z on |z| <= 1/2 by the cubic in z^2 through its values at the four
   // Chebyshev nodes of [0, 1/4]: tanh to 2.5e-7, relative 5.5e-7
   const double tanh_c[4] = {0.999999451, -0.3332628423, 0.1318993943, -0.04439273843};
   double f = cap_log2 * m->z_scale;
-  m->poly_range = m->z_scale > 0.f ? 0.5f / m->z_scale : -1.f;
+  // (up to 1e15, so that s^2 stays finite beside coefficients that vanish)
+  m->poly_range = m->z_scale > 0.f ? std::fmin(0.5f / m->z_scale, 1e15f) : -1.f;
   for (int i = 0; i < 4; ++i, f *= static_cast<double>(m->z_scale) * m->z_scale) {
     const double c = tanh_c[i] * f;
     m->poly[i] = static_cast<float>(c);
-    // scores so far from 1 that a coefficient leaves fp32: the other form
-    if (m->z_scale > 0.f && !(std::fabs(c) > 1e-35 && std::fabs(c) < 1e35)) m->poly_range = -1.f;
+    if (!(std::fabs(c) < 1e35)) m->poly_range = -1.f;  // a tiny cap: the other form
   }
   return MZ_OK;
 }

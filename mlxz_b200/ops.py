@@ -271,6 +271,8 @@ def paged_plan(block_tables: torch.Tensor, ctx_lens: torch.Tensor, q_lens: torch
             raise ValueError(f"{name} must hold one entry per sequence ({B})")
     if new_ids is not None and not _i32_on(new_ids, dev):
         _as_i32(new_ids, block_tables.device, "new_ids")
+    if width == 0 and B:
+        raise ValueError("block_tables must be [B, max_blocks] with max_blocks > 0")
     if n_rows < 0 or block_size < 1 or n_blocks < 1:
         raise ValueError("n_rows must be >= 0, block_size and n_blocks >= 1")
     dev = _dev_index(block_tables)
@@ -440,7 +442,7 @@ def decode_workspace(n_seqs: int, n_kv_heads: int, rows: int, head_dim: int, dev
     return _layout_workspace(_workspaces, key, int(size.value), device, shared)
 
 
-def _score_mod(n_heads: int, device: torch.device, softcap: float,
+def _score_mod(q: torch.Tensor, k_pool: torch.Tensor, n_heads: int, softcap: float,
                alibi_slopes: torch.Tensor | None, window: int, sink_tokens: int,
                prefix_lens: torch.Tensor | None, first_keys: torch.Tensor | None, n_seqs: int,
                n_first: int) -> "nat.ScoreMod | None":
@@ -450,18 +452,20 @@ def _score_mod(n_heads: int, device: torch.device, softcap: float,
         raise ValueError("softcap must be finite and not negative (0: none)")
     if window < 0 or sink_tokens < 0:
         raise ValueError("window and sink_tokens must not be negative")
-    if alibi_slopes is not None and (
-            alibi_slopes.dtype != torch.float32 or alibi_slopes.shape != (n_heads,) or
-            alibi_slopes.device != device or not alibi_slopes.is_contiguous()):
-        raise ValueError(f"alibi_slopes must be a contiguous float32 [{n_heads}] on {device}")
-    for t, name, n in ((prefix_lens, "prefix_lens", n_seqs), (first_keys, "first_keys", n_first)):
-        if t is not None:
-            _as_i32(t, device, name)
-            if t.numel() != n:
-                raise ValueError(f"{name} must hold {n} entries")
-    if not (softcap or window or alibi_slopes is not None or prefix_lens is not None
-            or first_keys is not None):
+    if not (softcap or window) and alibi_slopes is None and prefix_lens is None and \
+            first_keys is None:
         return None
+    dev = q.get_device()
+    if k_pool.get_device() != dev:
+        raise ValueError("q must be on the pools' device")
+    if alibi_slopes is not None and (
+            alibi_slopes.dtype is not torch.float32 or alibi_slopes.shape != (n_heads,) or
+            alibi_slopes.get_device() != dev or not alibi_slopes.is_contiguous()):
+        raise ValueError(f"alibi_slopes must be a contiguous float32 [{n_heads}] on {q.device}")
+    for t, name, n in ((prefix_lens, "prefix_lens", n_seqs), (first_keys, "first_keys", n_first)):
+        if t is not None and not (_i32_on(t, dev) and t.numel() == n):
+            _as_i32(t, q.device, name)
+            raise ValueError(f"{name} must hold {n} entries")
     big = (1 << 31) - 1
     return nat.ScoreMod(softcap, min(window, big), min(sink_tokens, big), _ptr(alibi_slopes),
                         _ptr(prefix_lens), _ptr(first_keys))
@@ -539,7 +543,7 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         o_sb, o_st, o_sh = out.stride(0), out.stride(1), out.stride(2)
     if scale is None:
         scale = D ** -0.5
-    mod = _score_mod(Hq, q.device, softcap, alibi_slopes, window, sink_tokens, prefix_lens,
+    mod = _score_mod(q, k_pool, Hq, softcap, alibi_slopes, window, sink_tokens, prefix_lens,
                      first_keys, B, B)
     if mod is not None and nq > 1 and not causal:
         raise ValueError("modified scores of several query tokens need causal=True")
@@ -606,8 +610,10 @@ def paged_append_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Ten
         raise ValueError("out must match q's shape with unit last stride")
     if scale is None:
         scale = D ** -0.5
-    mod = _score_mod(Hq, q.device, softcap, alibi_slopes, window, sink_tokens, prefix_lens,
+    mod = _score_mod(q, k_pool, Hq, softcap, alibi_slopes, window, sink_tokens, prefix_lens,
                      first_keys, B, B)
+    if mod is not None and not (k_new.get_device() == v_new.get_device() == q.get_device()):
+        raise ValueError("k_new and v_new must be on the pools' device")
     if B == 0:
         return out
     dev = _dev_index(q)
@@ -669,7 +675,7 @@ def paged_prefill(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         raise ValueError("out must match q's shape with unit last stride")
     if scale is None:
         scale = D ** -0.5
-    mod = _score_mod(Hq, q.device, softcap, alibi_slopes, window, sink_tokens, prefix_lens,
+    mod = _score_mod(q, k_pool, Hq, softcap, alibi_slopes, window, sink_tokens, prefix_lens,
                      first_keys, B, T)
     if B == 0 or T == 0 or max_q_len == 0:
         return out

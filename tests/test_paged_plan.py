@@ -211,6 +211,8 @@ def test_plan_refusals_on_the_host():
         ops.paged_plan(t, v, v, 4, 16, 8, held=v[:1])
     with pytest.raises(ValueError, match="n_rows"):
         ops.paged_plan(t, v, v, -1, 16, 8)
+    with pytest.raises(ValueError, match="max_blocks"):
+        ops.paged_plan(t[:, :0], v, v, 4, 16, 8)
 
 
 def test_plan_c_abi_argument_errors():

@@ -479,3 +479,60 @@ def test_default_workspaces_of_two_streams_and_of_two_graphs(cuda):
     ops.check_device_errors(0)
     for o in outs:
         _check(o, want)
+
+
+@gpu
+@pytest.mark.parametrize("softcap", [1e-6, 0.5, 1500.0, 3e4, 1e29, 1e32])
+def test_caps_of_every_size(cuda, softcap):
+    """From caps that bind every score to those that touch none; scores near and
+    far beyond softcap / 2 in the same tile.  Above 1000 the scores may be off by
+    2.4e-7 of the cap, doubled for numerator and row sum: that share of spread on
+    top where a score beyond half the cap is near (none at these sizes above
+    3e4)."""
+    dtype, D, G, ctx, qlen = "bf16", 64, 4, [130, 300], [70, 9]
+    case = _prefill_case(60, ctx, qlen, dtype, D, G, 16, 2)
+    # scores of standard deviation 8
+    case["qp"] = to_bits(8 * to_dev(case["qp"], dtype, "cpu"))
+    want = osm.paged(case["qp"], case["kp"], case["vp"], case["tables"], case["q_start"],
+                     case["q_len"], case["ctx"], dtype, softcap=softcap)
+    _check(_prefill(case, dtype, cuda, dict(softcap=softcap)), want)
+    kp, vp, tables, c = _dev(case, dtype, cuda)
+    last = case["q_start"] + case["q_len"] - 1
+    out = ops.paged_decode(to_dev(case["qp"][last], dtype, cuda), kp, vp, tables, c,
+                           softcap=softcap)
+    _check(out, (want[0][last], want[1][last]))
+    ops.check_device_errors(0)
+
+
+@gpu
+def test_nan_keys_and_queries_reach_their_rows_only(cuda):
+    """A NaN key poisons the rows that see it, a NaN query its own row."""
+    dtype, D, ctx = "bf16", 64, [40, 40]
+    case = _prefill_case(61, ctx, [40, 40], dtype, D, 2, 16, 1)
+    kp, vp, tables, c = _dev(case, dtype, cuda)
+    kp[int(tables[0, 2]), :, 3] = float("nan")  # key 35 of the first request
+    q = to_dev(case["qp"], dtype, cuda)
+    q[40 + 7, 1] = float("nan")
+    i = {k: torch.from_numpy(case[k]).to(cuda) for k in ("q_start", "q_len")}
+    kw = dict(window=4, softcap=20.0)
+    out = ops.paged_prefill(q, kp, vp, tables, i["q_start"], i["q_len"], c, 40, **kw)
+    bad = out.isnan().all(-1)
+    want = torch.zeros(80, 2, dtype=torch.bool)
+    want[35:39] = True
+    want[47, 1] = True
+    assert torch.equal(bad.cpu(), want) and torch.equal(out.isnan().any(-1), bad)
+    dec = ops.paged_decode(q[[38, 47]].contiguous(), kp, vp, tables, c - 1, **kw)
+    assert dec[0].isnan().all() and dec[1, 1].isnan().all() and not dec[1, 0].isnan().any()
+
+
+def test_caps_that_overflow_and_tables_too_wide_are_refused():
+    lib = _native.lib()
+    p = ctypes.c_void_p(64)
+
+    def append(width=2, **mod):
+        return lib.mz_paged_append_decode_mod(
+            p, 1, 512, 64, p, 512, 64, p, p, p, p, 128, 64, p, width, p, 1, 8, 2, 64, 16, 4, 0.125,
+            ctypes.byref(_native.ScoreMod(**mod)), 1, 0, 0, p, 0, None, None)
+
+    assert append(softcap=1e-40) == _native.MZ_ERR_INVALID_ARG
+    assert append(width=1 << 27, window=3) == _native.MZ_ERR_UNSUPPORTED
