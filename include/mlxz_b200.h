@@ -294,9 +294,8 @@ MZ_API int mz_paged_prefill(void *out, int32_t out_dtype, int64_t out_tok_stride
  * gets zeros.  Blocks that no token of the call sees are not read: their
  * table entries may be stale.  All arrays are on the device; like ctx_lens,
  * the kernel ahead of a launch with MZ_LAUNCH_OVERLAP_PREVIOUS must not write
- * them.  Scores are off by at most 2.4e-7 * softcap up to a cap of 1000 (above
- * it by 1e-6 of themselves, in a prefill tile with a score beyond softcap / 2
- * still by 2.4e-7 * softcap); a cap from 1e30 on is none.  Same
+ * them.  The cap is off by at most 2.4e-7 * softcap, above a cap of 1000 by 1e-6
+ * of the score; a cap from 1e30 on is none.  Same
  * place in the reference as the unmodified calls: the scaled dot product
  * attention of src/mlxz/paged_attention/attention.py:40-42, whose models mask
  * and cap; streaming_sink_size of src/mlxz/config.py:28-36 is sink_tokens. */

@@ -53,7 +53,6 @@ constexpr int kSoftWarps = 4;  // per stream
 constexpr int kThreads = 32 * kStreams * (kSoftWarps + 2);
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleLog2 = 8.f;
-constexpr int kPairs = 8;
 static_assert(kSlots == 2, "phases below count tiles by pairs");
 
 template <int D>
@@ -82,20 +81,49 @@ struct Item {
   __device__ __forceinline__ int own(int t) const { return t < head_tiles ? t : t + skip; }
 };
 
-// Item e, whole warps: a query block (the last, longest ones first) of a pair =
-// (sequence, KV head).  False: nothing to do.
-__device__ __forceinline__ bool item_at(const PParams &p, int e, Item &it) {
+// Where a stream's search for its next item stands: sequence b's first item is
+// `base`.
+struct Walk {
+  int b = 0, base = 0;
+};
+
+// Item e, whole warps.  Items are the query blocks that the sequences have, a
+// sequence's last (longest) ones first and its KV heads in turn, so that
+// neighbours in time share K/V through L2 without all reading the same tiles at
+// once, and a batch of ragged or empty chunks costs no empty items.  False: none
+// is left (*end), or the item's sequence is in error.
+__device__ __forceinline__ bool item_at(const PParams &p, Walk &w, int e, Item &it, bool *end) {
   const int lane = threadIdx.x & 31, tpc = kM / p.G;
-  // kPairs pairs at a time, their query blocks in turn: neighbours in time share
-  // K/V through L2 without all reading the same tiles at once
-  const int pairs = p.n_seqs * p.Hkv;
-  const int first = e / (kPairs * p.qblocks) * kPairs, np = min(kPairs, pairs - first);
-  const int r = e - first * p.qblocks, jr = r / np, pair = first + r - jr * np;
-  it.b = pair / p.Hkv;
-  it.h = pair - it.b * p.Hkv;
-  it.q0 = (p.qblocks - 1 - jr) * tpc;
-  const int n = p.q_len[it.b];
-  if (n <= 0 || it.q0 >= n) return false;
+  int n = 0, blocks = 0;
+  for (;; w.b += 32) {
+    if (w.b >= p.n_seqs) {
+      *end = true;
+      return false;
+    }
+    const int b = w.b + lane;
+    n = b < p.n_seqs ? max(0, p.q_len[b]) : 0;
+    blocks = min((n + tpc - 1) / tpc, p.qblocks);
+    const int mine = blocks * p.Hkv;
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += y;
+    }
+    const unsigned found = __ballot_sync(0xffffffffu, w.base + incl > e);
+    const int from = found ? __ffs(found) - 1 : 31;
+    w.base += __shfl_sync(0xffffffffu, found ? incl - mine : incl, from);
+    if (found) {
+      w.b += from;
+      n = __shfl_sync(0xffffffffu, n, from);
+      blocks = __shfl_sync(0xffffffffu, blocks, from);
+      break;
+    }
+  }
+  it.b = w.b;
+  const int r = e - w.base, jr = r / p.Hkv;
+  it.h = r - jr * p.Hkv;
+  it.q0 = (blocks - 1 - jr) * tpc;
   const int ctx = p.ctx[it.b];
   if (ctx < n || ctx > (int64_t)p.max_blocks * p.bs) {
     if (lane == 0) dev_error(p.err, MZ_DEVERR_CONTEXT);
@@ -186,12 +214,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // Items go to the streams in turn, all first streams before all second ones:
   // in the last round they spread over the SMs.
-  const int n_items = p.n_seqs * p.Hkv * p.qblocks;
   const int e0 = st * gridDim.x + blockIdx.x, e_step = kStreams * gridDim.x;
+  Walk walk;
   auto next_item = [&](int &e, Item &it) {
-    for (; e < n_items; e += e_step)
-      if (item_at(p, e, it)) return true;
-    return false;
+    for (bool end = false;; e += e_step) {
+      if (item_at(p, walk, e, it, &end)) return true;
+      if (end) return false;
+    }
   };
   auto give_up = [&]() {
     dev_error(p.err, MZ_DEVERR_TIMEOUT);
@@ -400,13 +429,37 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int x = 0; x < kN; ++x) sv[x] = __uint_as_float(r[x >> 5][x & 31]);
         }
         const int key0 = tile * kN;
+        // whether the tile crosses a border of what the row sees, and which of its
+        // keys are hidden then
+        const bool edge = !((key0 >= lo && key0 + kN - 1 <= pos) || key0 + kN <= head);
+        auto hidden = [&](int x) {
+          const int key = key0 + x;
+          return key >= head && (key > pos || key < lo);
+        };
         if constexpr (MODE > 2) {
+          // hidden keys may be anything and must not choose the form below
+          if (edge) {
+#pragma unroll
+            for (int x = 0; x < kN; ++x)
+              if (hidden(x)) sv[x] = 0.f;
+          }
           float big = fmax3f(fabsf(sv[0]), fabsf(sv[1]), 0.f);
 #pragma unroll
           for (int x = 2; x < kN; x += 2) big = fmax3f(big, fabsf(sv[x]), fabsf(sv[x + 1]));
           if (__any_sync(0xffffffffu, !(big <= p.mod.poly_range))) {
+            if (p.mod.cap_log2 <= kQuickCapLog2) {
 #pragma unroll
-            for (int x = 0; x < kN; ++x) sv[x] = cap_quick(p.mod, sv[x]);
+              for (int x = 0; x < kN; ++x) sv[x] = cap_quick(p.mod, sv[x]);
+            } else {
+              // the quick form's error grows with the cap: for large scores alone
+#pragma unroll
+              for (int x = 0; x < kN; ++x) {
+                const float w = sv[x] * sv[x];
+                const float y = fmaf(fmaf(fmaf(w, p.mod.poly[3], p.mod.poly[2]), w, p.mod.poly[1]),
+                                     w, p.mod.poly[0]) * sv[x];
+                sv[x] = fabsf(sv[x]) <= p.mod.poly_range ? y : cap_quick(p.mod, sv[x]);
+              }
+            }
           } else {
             const uint64_t c0 = f2_pack(p.mod.poly[0], p.mod.poly[0]),
                            c1 = f2_pack(p.mod.poly[1], p.mod.poly[1]),
@@ -439,13 +492,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               sv[x] = fmaf(-slope, fabsf(far + static_cast<float>(x)), MODE > 2 ? sv[x] : sv[x] * sc);
           }
         }
-        if (!((key0 >= lo && key0 + kN - 1 <= pos) || key0 + kN <= head)) {
-          // this tile crosses a border of what the row sees
+        if (edge) {
 #pragma unroll
-          for (int x = 0; x < kN; ++x) {
-            const int key = key0 + x;
-            if (key >= head && (key > pos || key < lo)) sv[x] = -INFINITY;
-          }
+          for (int x = 0; x < kN; ++x)
+            if (hidden(x)) sv[x] = -INFINITY;
         }
         // maximum: four independent chains of three-input maxima
         float m4[4];

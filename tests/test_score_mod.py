@@ -484,11 +484,8 @@ def test_default_workspaces_of_two_streams_and_of_two_graphs(cuda):
 @gpu
 @pytest.mark.parametrize("softcap", [1e-6, 0.5, 1500.0, 3e4, 1e29, 1e32])
 def test_caps_of_every_size(cuda, softcap):
-    """From caps that bind every score to those that touch none; scores near and
-    far beyond softcap / 2 in the same tile.  Above 1000 the scores may be off by
-    2.4e-7 of the cap, doubled for numerator and row sum: that share of spread on
-    top where a score beyond half the cap is near (none at these sizes above
-    3e4)."""
+    """From caps that bind every score to those that touch none, with scores near
+    and far beyond half the cap in the same tile."""
     dtype, D, G, ctx, qlen = "bf16", 64, 4, [130, 300], [70, 9]
     case = _prefill_case(60, ctx, qlen, dtype, D, G, 16, 2)
     # scores of standard deviation 8
@@ -536,3 +533,21 @@ def test_caps_that_overflow_and_tables_too_wide_are_refused():
 
     assert append(softcap=1e-40) == _native.MZ_ERR_INVALID_ARG
     assert append(width=1 << 27, window=3) == _native.MZ_ERR_UNSUPPORTED
+
+
+@gpu
+@pytest.mark.parametrize("softcap", [20.0, 3e4, 1e29])
+def test_capped_prefill_ignores_what_lies_behind_the_last_key(cuda, softcap):
+    """The last tile's rows behind the sequence are whatever the block holds:
+    huge values there change no byte."""
+    dtype, D, G, ctx, qlen = "bf16", 64, 4, [130, 300], [70, 9]
+    case = _prefill_case(62, ctx, qlen, dtype, D, G, 16, 2)
+    want = _prefill(case, dtype, cuda, dict(softcap=softcap))
+    kp, vp, tables, c = _dev(case, dtype, cuda)
+    for b, n in enumerate(ctx):
+        for fill in (3e38, float("nan"), float("-inf")):
+            blk = int(tables[b, (n - 1) // 16])
+            kp[blk, :, n % 16:] = fill
+            vp[blk, :, n % 16:] = fill
+            got = _prefill(case, dtype, cuda, dict(softcap=softcap), pools=(kp, vp, tables, c))
+            assert torch.equal(got, want)
