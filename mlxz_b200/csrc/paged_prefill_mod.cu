@@ -436,31 +436,59 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int key = key0 + x;
           return key >= head && (key > pos || key < lo);
         };
+        float top = 0.f;  // MODE 3: no score of the tile is above it
         if constexpr (MODE > 2) {
-          // hidden keys may be anything and must not choose the form below
-          if (edge) {
-#pragma unroll
-            for (int x = 0; x < kN; ++x)
-              if (hidden(x)) sv[x] = 0.f;
-          }
           float big = fmax3f(fabsf(sv[0]), fabsf(sv[1]), 0.f);
 #pragma unroll
           for (int x = 2; x < kN; x += 2) big = fmax3f(big, fabsf(sv[x]), fabsf(sv[x + 1]));
-          if (__any_sync(0xffffffffu, !(big <= p.mod.poly_range))) {
-            if (p.mod.cap_log2 <= kQuickCapLog2) {
+          bool small = __all_sync(0xffffffffu, big <= p.mod.poly_range);
+          if (!small) {
+            // sixteen scores at a time in TMEM: little code for what few tiles need.
+            // Hidden keys may be anything: they must not choose the form.
+            big = 0.f;
+#pragma unroll 1
+            for (int c = 0; c < kN / 16; ++c) {
+              uint32_t r[16];
+              tc::ld16(scol + 16 * c, r);
+              tc::wait_ld();
 #pragma unroll
-              for (int x = 0; x < kN; ++x) sv[x] = cap_quick(p.mod, sv[x]);
-            } else {
-              // the quick form's error grows with the cap: for large scores alone
-#pragma unroll
-              for (int x = 0; x < kN; ++x) {
-                const float w = sv[x] * sv[x];
-                const float y = fmaf(fmaf(fmaf(w, p.mod.poly[3], p.mod.poly[2]), w, p.mod.poly[1]),
-                                     w, p.mod.poly[0]) * sv[x];
-                sv[x] = fabsf(sv[x]) <= p.mod.poly_range ? y : cap_quick(p.mod, sv[x]);
+              for (int x = 0; x < 16; ++x) {
+                if (edge && hidden(16 * c + x)) r[x] = 0u;
+                big = fmaxf(big, fabsf(__uint_as_float(r[x])));
               }
+              tc::st16(scol + 16 * c, r);
             }
-          } else {
+            tc::wait_st();
+            small = __all_sync(0xffffffffu, big <= p.mod.poly_range);
+            if (!small) {
+#pragma unroll 1
+              for (int c = 0; c < kN / 16; ++c) {
+                uint32_t r[16];
+                tc::ld16(scol + 16 * c, r);
+                tc::wait_ld();
+#pragma unroll
+                for (int x = 0; x < 16; ++x) {
+                  const float v = __uint_as_float(r[x]);
+                  float y = cap_quick(p.mod, v);
+                  // its error grows with the cap: above 1000 for large scores alone
+                  if (p.mod.cap_log2 > kQuickCapLog2 && fabsf(v) <= p.mod.poly_range)
+                    y = cap_poly(p.mod, v);
+                  r[x] = __float_as_uint(y);
+                }
+                tc::st16(scol + 16 * c, r);
+              }
+              tc::wait_st();
+            }
+            uint32_t r[2][32];
+            tc::ld32(scol, r[0]);
+            tc::ld32(scol + 32, r[1]);
+            tc::wait_ld();
+#pragma unroll
+            for (int x = 0; x < kN; ++x) sv[x] = __uint_as_float(r[x >> 5][x & 31]);
+          }
+          top = p.mod.cap_log2;
+          if (small) {
+            top = cap_poly(p.mod, big);
             const uint64_t c0 = f2_pack(p.mod.poly[0], p.mod.poly[0]),
                            c1 = f2_pack(p.mod.poly[1], p.mod.poly[1]),
                            c2 = f2_pack(p.mod.poly[2], p.mod.poly[2]),
@@ -472,6 +500,9 @@ __global__ void __launch_bounds__(kThreads, 1)
               f2_unpack(f2_mul(y, v), sv[x], sv[x + 1]);
             }
           }
+          // (slopes below 0 raise scores with the distance)
+          top += fmaxf(0.f, -slope) * fmaxf(fabsf(static_cast<float>(key0 - pos)),
+                                            fabsf(static_cast<float>(key0 + kN - 1 - pos)));
         }
         if constexpr (MODE > 1) {
           const float far = static_cast<float>(key0 - pos);
@@ -497,20 +528,26 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int x = 0; x < kN; ++x)
             if (hidden(x)) sv[x] = -INFINITY;
         }
-        // maximum: four independent chains of three-input maxima
-        float m4[4];
+        // the tile's maximum, in four independent chains of three-input maxima; with
+        // a cap only where the bound on it exceeds m by more than 8
+        bool need = false;
+        float m_new = m_used, alpha = 1.f;
+        if (MODE < 3 || __any_sync(0xffffffffu, top > m_used + kRescaleLog2)) {
+          float m4[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          float m = fmax3f(sv[k], sv[k + 4], sv[k + 8]);
+          for (int k = 0; k < 4; ++k) {
+            float m = fmax3f(sv[k], sv[k + 4], sv[k + 8]);
 #pragma unroll
-          for (int t = 3; t + 1 < kN / 4; t += 2) m = fmax3f(m, sv[k + 4 * t], sv[k + 4 * (t + 1)]);
-          m4[k] = fmaxf(m, sv[k + kN - 4]);
+            for (int t = 3; t + 1 < kN / 4; t += 2)
+              m = fmax3f(m, sv[k + 4 * t], sv[k + 4 * (t + 1)]);
+            m4[k] = fmaxf(m, sv[k + kN - 4]);
+          }
+          float mx = fmax3f(m4[0], m4[1], fmaxf(m4[2], m4[3]));
+          if constexpr (MODE < 2) mx *= p.scale_log2;  // scale > 0
+          need = mx > m_used + kRescaleLog2;
+          m_new = need ? mx : m_used;
+          alpha = need ? fast_exp2(m_used - m_new) : 1.f;
         }
-        float mx = fmax3f(m4[0], m4[1], fmaxf(m4[2], m4[3]));
-        if constexpr (MODE < 2) mx *= p.scale_log2;  // scale > 0
-        const bool need = mx > m_used + kRescaleLog2;
-        const float m_new = need ? mx : m_used;
-        const float alpha = need ? fast_exp2(m_used - m_new) : 1.f;
         if (i > 0 && __any_sync(0xffffffffu, need)) {
           // O holds P.V up to tile i - 1: S_i was issued after P.V of tile i - 2
           if (!wait(kBarPvDone + ((j - 1) & 1), (j - 1) >> 1)) {

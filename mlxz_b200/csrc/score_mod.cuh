@@ -60,6 +60,10 @@ __device__ __forceinline__ float cap_quick(const ScoreMod &m, float s) {
   return fmaf(-2.f * m.cap_log2, rcp_approx(fast_exp2(s * (m.z_scale * (2.f * kLog2e))) + 1.f),
               m.cap_log2);
 }
+__device__ __forceinline__ float cap_poly(const ScoreMod &m, float s) {
+  const float w = s * s;
+  return fmaf(fmaf(fmaf(w, m.poly[3], m.poly[2]), w, m.poly[1]), w, m.poly[0]) * s;
+}
 constexpr float kQuickCapLog2 = 1000.f * kLog2e;
 
 // Host side: the fields of mz_score_mod checked and folded with the scale.

@@ -551,3 +551,20 @@ def test_capped_prefill_ignores_what_lies_behind_the_last_key(cuda, softcap):
             vp[blk, :, n % 16:] = fill
             got = _prefill(case, dtype, cuda, dict(softcap=softcap), pools=(kp, vp, tables, c))
             assert torch.equal(got, want)
+
+
+@gpu
+@pytest.mark.parametrize("softcap", [0.0, 5.0, 30.0])
+def test_negative_slopes_raise_far_scores(cuda, softcap):
+    """Slopes below 0: scores grow with the distance, beyond the cap."""
+    dtype, D, G, ctx, qlen = "bf16", 64, 2, [700, 130], [90, 130]
+    case = _prefill_case(63, ctx, qlen, dtype, D, G, 16, 2)
+    s = np.array([-0.25, -0.01, 0.0, 0.5], dtype=np.float32)
+    kw = dict(softcap=softcap, alibi_slopes=torch.from_numpy(s).to(cuda))
+    want = osm.paged(case["qp"], case["kp"], case["vp"], case["tables"], case["q_start"],
+                     case["q_len"], case["ctx"], dtype, softcap=softcap, slopes=s)
+    _check(_prefill(case, dtype, cuda, kw), want)
+    kp, vp, tables, c = _dev(case, dtype, cuda)
+    last = case["q_start"] + case["q_len"] - 1
+    out = ops.paged_decode(to_dev(case["qp"][last], dtype, cuda), kp, vp, tables, c, **kw)
+    _check(out, (want[0][last], want[1][last]))
