@@ -136,8 +136,11 @@ class PagedPrefillStep:
         self.max_q_len = max([0] + [n for _, n in self.chunks])
         self.tables = tables.to(dev)
         cached, self.q_len, held = lens.to(dev)
-        plan = ops.paged_plan(self.tables, cached, self.q_len, self.T, store.block_size,
-                              store.n_blocks, held=held)
+        if dev.type == "cuda":
+            plan = ops.paged_plan(self.tables, cached, self.q_len, self.T, store.block_size,
+                                  store.n_blocks, held=held)
+        else:  # a store without a GPU: metadata alone, no layer runs
+            plan = self._host_plan(lens)
         self.q_start, self.ctx_lens, self.slots = plan.q_start, plan.lengths, plan.slots
         self.positions = plan.positions
         self.rope_positions = self.positions if rope_positions is None else rope_positions
@@ -157,6 +160,19 @@ class PagedPrefillStep:
         self._ids = torch.tensor(uniq, dtype=torch.int32).to(dev) if self.quantized else None
         self._stage = None
         self._done = False
+
+    def _host_plan(self, lens: torch.Tensor) -> ops.PagedPlan:
+        """What ops.paged_plan gives for these lengths, on the host."""
+        bs = self.store.block_size
+        cached, new, held = lens
+        starts = torch.cumsum(new, 0, dtype=torch.int32) - new
+        pos = [p for c, n in zip(cached.tolist(), new.tolist()) for p in range(c, c + n)]
+        blocks = [self.store.tables[s][p // bs] for (s, n), c in zip(self.chunks, cached.tolist())
+                  for p in range(c, c + n)]
+        positions = torch.tensor(pos, dtype=torch.int32)
+        slots = torch.tensor(blocks, dtype=torch.int64) * bs + positions % bs
+        return ops.PagedPlan(starts, positions, slots, cached + new, held,
+                             torch.zeros(1, dtype=torch.int32))
 
     def layer(self, l: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
               out: torch.Tensor | None = None, out_dtype: torch.dtype | None = None

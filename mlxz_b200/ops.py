@@ -117,13 +117,14 @@ def _i32_on(t: torch.Tensor, dev: int) -> bool:
 
 
 def _check_pools(k_pool: torch.Tensor, v_pool: torch.Tensor) -> tuple[int, int, int, int]:
-    if k_pool.shape != v_pool.shape or k_pool.dtype != v_pool.dtype:
+    shape = k_pool.shape
+    if shape != v_pool.shape or k_pool.dtype is not v_pool.dtype:
         raise ValueError("k_pool and v_pool must have the same shape and dtype")
-    if k_pool.dim() != 4 or not k_pool.is_contiguous() or not v_pool.is_contiguous():
+    if len(shape) != 4 or not k_pool.is_contiguous() or not v_pool.is_contiguous():
         raise ValueError("pools must be contiguous [n_blocks, n_kv_heads, block_size, head_dim]")
-    if k_pool.device != v_pool.device:
+    if k_pool.get_device() != v_pool.get_device():
         raise ValueError("pools must be on the same device")
-    n, h, bs, d = k_pool.shape
+    n, h, bs, d = shape
     return n, h, bs, d
 
 
@@ -528,13 +529,15 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         raise ValueError(f"q head_dim must be {D} with unit stride")
     if Hq % Hkv:
         raise ValueError(f"n_heads {Hq} is not a multiple of n_kv_heads {Hkv}")
-    _as_i32(block_tables, k_pool.device, "block_tables")
-    _as_i32(ctx_lens, k_pool.device, "ctx_lens")
+    dev = k_pool.get_device()
+    if not (_i32_on(block_tables, dev) and _i32_on(ctx_lens, dev)):
+        _as_i32(block_tables, k_pool.device, "block_tables")
+        _as_i32(ctx_lens, k_pool.device, "ctx_lens")
     if block_tables.dim() != 2 or block_tables.shape[0] < B or ctx_lens.numel() < B:
         raise ValueError("block_tables must be [>=B, max_blocks] and ctx_lens [>=B]")
     out_dtype = out_dtype or q.dtype
     if out is None:
-        out = torch.empty(q.shape, dtype=out_dtype, device=q.device)
+        out = q.new_empty(q.shape, dtype=out_dtype)
     if out.shape != q.shape or out.dtype != out_dtype or out.stride(-1) != 1:
         raise ValueError("out must match q's shape with unit last stride")
     if q.dim() == 3:
@@ -601,11 +604,13 @@ def paged_append_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Ten
         raise ValueError("k_new/v_new dtype must match the pools")
     if k_new.stride() != v_new.stride() or k_new.stride(2) != 1:
         k_new, v_new = k_new.contiguous(), v_new.contiguous()
-    _as_i32(block_tables, k_pool.device, "block_tables")
-    _as_i32(ctx_lens, k_pool.device, "ctx_lens")
+    dev = k_pool.get_device()
+    if not (_i32_on(block_tables, dev) and _i32_on(ctx_lens, dev)):
+        _as_i32(block_tables, k_pool.device, "block_tables")
+        _as_i32(ctx_lens, k_pool.device, "ctx_lens")
     out_dtype = out_dtype or q.dtype
     if out is None:
-        out = torch.empty(q.shape, dtype=out_dtype, device=q.device)
+        out = q.new_empty(q.shape, dtype=out_dtype)
     if out.shape != q.shape or out.dtype != out_dtype or out.stride(-1) != 1:
         raise ValueError("out must match q's shape with unit last stride")
     if scale is None:
@@ -670,7 +675,7 @@ def paged_prefill(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     _as_i32(block_tables, k_pool.device, "block_tables")
     out_dtype = out_dtype or q.dtype
     if out is None:
-        out = torch.empty(q.shape, dtype=out_dtype, device=q.device)
+        out = q.new_empty(q.shape, dtype=out_dtype)
     if out.shape != q.shape or out.dtype != out_dtype or out.stride(-1) != 1:
         raise ValueError("out must match q's shape with unit last stride")
     if scale is None:
