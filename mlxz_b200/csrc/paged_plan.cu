@@ -25,19 +25,24 @@ constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kRowsPerThread = 4;
 constexpr int kRows = kThreads * kRowsPerThread;  // rows of a CTA
-constexpr int kSeqs = 8;                          // sequences per thread and round
+constexpr int kSeqs = 8;                          // most sequences per thread and round
 
 struct PlanParams {
   int32_t *tables;
   int max_blocks;
   const int32_t *ctx, *q, *held, *new_ids;
   int n_new, B, n_rows, bs;
+  int bs_log2;  // -1: no power of two
   int64_t n_blocks;
   int32_t *q_start, *positions;
   int64_t *slots;
   int32_t *lengths, *held_out, *n_used;
   int32_t *err;
 };
+
+__device__ __forceinline__ int blocks_below(const PlanParams &p, int tokens) {
+  return p.bs_log2 >= 0 ? tokens >> p.bs_log2 : tokens / p.bs;
+}
 
 // A sequence's checked lengths: q = 0 where they do not fit its table.
 struct Seq {
@@ -49,12 +54,13 @@ __device__ __forceinline__ Seq read_seq(const PlanParams &p, int b) {
   Seq s;
   s.ctx = p.ctx[b];
   s.q = p.q[b];
-  s.held = p.held ? p.held[b] : (max(s.ctx, 0) + p.bs - 1) / p.bs;
   const int64_t end = (int64_t)s.ctx + s.q;
-  s.ok = s.ctx >= 0 && s.q >= 0 && end <= (int64_t)p.max_blocks * p.bs && s.held >= 0 &&
-         s.held <= p.max_blocks && (int64_t)s.held * p.bs >= s.ctx;
+  s.ok = s.ctx >= 0 && s.q >= 0 && end <= (int64_t)p.max_blocks * p.bs;  // < 2^31
+  // ceil(x / bs) = floor((x - 1) / bs) + 1 for x > 0: no sum that could overflow
+  s.held = p.held ? p.held[b] : s.ctx > 0 ? blocks_below(p, s.ctx - 1) + 1 : 0;
+  s.ok = s.ok && s.held >= 0 && s.held <= p.max_blocks && (int64_t)s.held * p.bs >= s.ctx;
   if (!s.ok) s.q = 0;
-  s.need = s.ok ? max(0, static_cast<int>((end + p.bs - 1) / p.bs) - s.held) : 0;
+  s.need = s.ok && end > 0 ? max(0, blocks_below(p, static_cast<int>(end) - 1) + 1 - s.held) : 0;
   return s;
 }
 
@@ -62,7 +68,9 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(const PlanParams p
   __shared__ int64_t w_rows[kWarps];
   __shared__ int w_need[kWarps];
   __shared__ int w_mark[kWarps];
-  __shared__ int s_seq[kRows], s_start[kRows], s_base[kRows];  // at a sequence's first row here
+  // at a sequence's first row here: the sequence, the position of row 0 of this
+  // block in it, its blocks, and where its new ones start
+  __shared__ int s_seq[kRows], s_pos[kRows], s_held[kRows], s_base[kRows];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t r0 = (int64_t)blockIdx.x * kRows;
   const int64_t r1 = min(r0 + kRows, (int64_t)p.n_rows);
@@ -71,15 +79,16 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(const PlanParams p
 
   int64_t rows0 = 0;  // rows and new blocks of the sequences of earlier rounds
   int need0 = 0;
-  for (int b0 = 0; b0 < p.B; b0 += kThreads * kSeqs) {
+  const int per = min(kSeqs, (p.B + kThreads - 1) / kThreads);  // sequences per thread
+  for (int b0 = 0; b0 < p.B; b0 += kThreads * per) {
     Seq s[kSeqs];
     int64_t rows = 0;
     int need = 0;
-    const int bt = b0 + threadIdx.x * kSeqs;
+    const int bt = b0 + threadIdx.x * per;
 #pragma unroll
     for (int k = 0; k < kSeqs; ++k) {
       s[k] = Seq{0, 0, 0, 0, true};
-      if (bt + k < p.B) s[k] = read_seq(p, bt + k);
+      if (k < per && bt + k < p.B) s[k] = read_seq(p, bt + k);
       rows += s[k].q;
       need += s[k].need;
     }
@@ -113,6 +122,7 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(const PlanParams p
 #pragma unroll
     for (int k = 0; k < kSeqs; ++k) {
       const int b = bt + k;
+      if (k >= per) break;
       if (b < p.B) {
         const bool fits = start + s[k].q <= p.n_rows;
         const int got = min(s[k].need, max(0, p.n_new - base));
@@ -128,7 +138,8 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(const PlanParams p
         if (fits && s[k].q > 0 && start < r1 && start + s[k].q > r0) {
           const int i = static_cast<int>(max(start, r0) - r0);
           s_seq[i] = b;
-          s_start[i] = static_cast<int>(start - r0);
+          s_pos[i] = s[k].ctx + static_cast<int>(r0 - start);
+          s_held[i] = s[k].held;
           s_base[i] = base;
         } else if (!fits && start >= r0 && start < r1) {
           s_seq[static_cast<int>(start - r0)] = p.B;  // no sequence from here on
@@ -173,12 +184,12 @@ __global__ void __launch_bounds__(kThreads) paged_plan_kernel(const PlanParams p
     int64_t slot = -1;
     const int b = at >= 0 ? s_seq[at] : p.B;
     if (b < p.B) {
-      const Seq s = read_seq(p, b);
-      pos = s.ctx + (i - s_start[at]);
-      const int j = pos / p.bs, in = pos - j * p.bs;
+      const int held = s_held[at];
+      pos = s_pos[at] + i;
+      const int j = blocks_below(p, pos), in = pos - j * p.bs;
       int32_t id = -1;
-      if (j >= s.held) {
-        const int64_t x = (int64_t)s_base[at] + (j - s.held);
+      if (j >= held) {
+        const int64_t x = (int64_t)s_base[at] + (j - held);
         if (x < p.n_new) id = p.new_ids[x];
         if (id < 0 || id >= p.n_blocks) {
           if (x < p.n_new) dev_error(p.err, MZ_DEVERR_BLOCK_ID);
@@ -233,6 +244,9 @@ extern "C" int mz_paged_plan(int32_t *block_tables, int32_t max_blocks_per_seq,
   p.B = n_seqs;
   p.n_rows = n_rows;
   p.bs = block_size;
+  p.bs_log2 = -1;
+  for (int i = 0; i < 31; ++i)
+    if (block_size == 1 << i) p.bs_log2 = i;
   p.n_blocks = n_blocks;
   p.q_start = q_start;
   p.positions = positions;

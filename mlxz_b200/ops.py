@@ -36,6 +36,11 @@ _qworkspaces: "OrderedDict[tuple, torch.Tensor]" = OrderedDict()
 
 def _layout_workspace(cache, key: tuple, need: int, device: int, shared: bool) -> torch.Tensor:
     if not shared:
+        if torch.cuda.is_current_stream_capturing():
+            # its clearing runs with every replay: the counters at the front alone
+            ws = torch.empty(max(need, 256), dtype=torch.uint8, device=f"cuda:{device}")
+            ws[:4 * (key[1] * key[2] + 2)].zero_()
+            return ws
         return torch.zeros(max(need, 256), dtype=torch.uint8, device=f"cuda:{device}")
     ws = cache.get(key)
     if ws is None:
