@@ -231,7 +231,8 @@ class PagedDecodeStep:
         self.tables.copy_(host, non_blocking=False)
         self.positions.copy_(offs)
         self.lengths.copy_(offs + 1)
-        # blocks of each table that the device has
+        # offsets and blocks of each table that the device has
+        self._offsets = offs.tolist()
         self._uploaded = [len(self.store.tables[s]) for s in self.seq_ids]
         self._held = torch.tensor(self._uploaded, dtype=torch.int32).to(self.store.device)
 
@@ -305,10 +306,12 @@ class PagedDecodeStep:
             had = len(st.tables[s])
             st.ensure_capacity(s, 1)
             new += st.tables[s][had:]
-            in_step &= had == self._uploaded[i] and len(st.tables[s]) <= self.max_blocks
+            in_step &= (had == self._uploaded[i] and st.offsets[s] == self._offsets[i] + 1
+                        and len(st.tables[s]) <= self.max_blocks)
         if new and not in_step:
             self.sync_metadata()
             return
+        self._offsets = [o + 1 for o in self._offsets]
         self.positions.add_(1)
         self.lengths.add_(1)
         if new:

@@ -187,6 +187,21 @@ def test_advance_with_blocks_from_outside_and_outgrown_tables(cuda):
             step.advance()
 
 
+@gpu
+def test_advance_with_offsets_from_outside(cuda):
+    """Offsets that moved between steps go up with the next block."""
+    store = PagedKVStore(1, 32, HKV, D, BS, torch.bfloat16, cuda)
+    store.add_sequence("a", 15)
+    store.add_sequence("b", 3)
+    step = PagedDecodeStep(store, ["a", "b"], HQ, max_blocks=4)
+    store.offsets["b"] += 4
+    step.advance()  # "a" grows
+    assert step.positions.tolist() == [16, 8] and step.lengths.tolist() == [17, 9]
+    for i, s in enumerate(("a", "b")):
+        tb = store.tables[s]
+        assert step.tables[i].tolist() == tb + [-1] * (4 - len(tb))
+
+
 def test_fused_all_gather_takes_plain_steps_only():
     class Step:
         plain = False
