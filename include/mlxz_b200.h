@@ -310,7 +310,8 @@ typedef struct mz_score_mod {
 
 /* mz_paged_decode with modified scores and masks.  Unlike there, n_q_tokens > 1
  * tokens are the sequence's last ones (drafted tokens, their K/V appended):
- * token i is at position ctx_lens[b] - n_q_tokens + i (below 0: zeros).
+ * token i is at position ctx_lens[b] - n_q_tokens + i (below 0 it sees the
+ * prefix alone).
  * Arguments and rules otherwise as mz_paged_decode. */
 MZ_API int mz_paged_decode_mod(void *out, int32_t out_dtype, int64_t out_seq_stride,
                                int64_t out_tok_stride, int64_t out_head_stride, const void *q,

@@ -103,7 +103,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
       const int t = own_tile(p, c.b, c.t, c.n, c.ctx);
       int32_t blk = p.tables[(int64_t)c.b * p.max_blocks + t / p.tpb];
       if (blk < 0 || blk >= p.n_blocks) {
-        dev_error(p.err, MZ_DEVERR_BLOCK_ID);
+        // the last tile is read even where no row sees it: any block will do then
+        const MaskSpan m = mask_span(p, c.b, c.ctx);
+        if (p.kn || t * kTileTok < m.head || (t + 1) * kTileTok > m.lo)
+          dev_error(p.err, MZ_DEVERR_BLOCK_ID);
         blk = 0;
       }
       const int y = static_cast<int>(((int64_t)blk * p.Hkv + c.h) * p.bs + (t % p.tpb) * kTileTok);
@@ -161,8 +164,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
       p_min = cc.ctx - p.n_q;
       // lower ends rise with the token where the window sets them
       const int first = p.mod.first ? max(0, p.mod.first[cc.b]) : 0;
-      const int w = p.mod.window > 0 ? p.mod.window : 1 << 30;
-      lo_max = max(first, cc.ctx - w);
+      lo_max = p.mod.window > 0 ? max(first, cc.ctx - p.mod.window) : first;
 #pragma unroll
       for (int x = 0; x < RG; ++x) {
 #pragma unroll
@@ -171,7 +173,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
           m[x][y] = kNoMax;
           l[x][y] = 0.f;
           pos[x][y] = p_min + r / p.G;
-          lo[x][y] = max(first, pos[x][y] - w + 1);
+          lo[x][y] = p.mod.window > 0 ? max(first, pos[x][y] - p.mod.window + 1) : first;
           slope[x][y] = p.mod.slopes && r < p.rows ? p.mod.slopes[cc.h * p.G + r % p.G] * kLog2e : 0.f;
         }
         const auto *q16 = static_cast<const uint16_t *>(p.q);

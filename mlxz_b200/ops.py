@@ -279,8 +279,9 @@ def paged_plan(block_tables: torch.Tensor, ctx_lens: torch.Tensor, q_lens: torch
         _as_i32(new_ids, block_tables.device, "new_ids")
     if width == 0 and B:
         raise ValueError("block_tables must be [B, max_blocks] with max_blocks > 0")
-    if n_rows < 0 or block_size < 1 or n_blocks < 1:
-        raise ValueError("n_rows must be >= 0, block_size and n_blocks >= 1")
+    if not 0 <= n_rows < 1 << 31 or not 1 <= block_size < 1 << 31 or n_blocks < 1:
+        raise ValueError("n_rows must be >= 0, block_size and n_blocks >= 1, the first two "
+                         "below 2^31")
     dev = _dev_index(block_tables)
     positions, q_start, lengths, held_out, n_new = block_tables.new_empty(
         n_rows + 3 * B + 1).split_with_sizes((n_rows, B, B, B, 1))
@@ -380,8 +381,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
     T, Hq, D = q.shape
     Hkv = k.shape[1]
     qo_at, ko_at = _heads(q_out, "q_out", q, Hq), _heads(k_out, "k_out", q, Hkv)
-    _call(_dev_index(q), "mz_qk_norm_rope", *qo_at, *ko_at, *q_at, *k_at, None, 0, 0, None, None, None, 0, 0, *args,
-          T, Hq, Hkv, D, dtype_code(q.dtype))
+    _call(_dev_index(q), "mz_qk_norm_rope", *qo_at, *ko_at, *q_at, *k_at,
+          None, 0, 0, None, None, None, 0, 0, *args, T, Hq, Hkv, D, dtype_code(q.dtype))
     return q_out, k_out
 
 
@@ -448,7 +449,7 @@ def decode_workspace(n_seqs: int, n_kv_heads: int, rows: int, head_dim: int, dev
     return _layout_workspace(_workspaces, key, int(size.value), device, shared)
 
 
-def _score_mod(q: torch.Tensor, k_pool: torch.Tensor, n_heads: int, softcap: float,
+def _score_mod(q: torch.Tensor, n_heads: int, softcap: float,
                alibi_slopes: torch.Tensor | None, window: int, sink_tokens: int,
                prefix_lens: torch.Tensor | None, first_keys: torch.Tensor | None, n_seqs: int,
                n_first: int) -> "nat.ScoreMod | None":
@@ -462,8 +463,6 @@ def _score_mod(q: torch.Tensor, k_pool: torch.Tensor, n_heads: int, softcap: flo
             first_keys is None:
         return None
     dev = q.get_device()
-    if k_pool.get_device() != dev:
-        raise ValueError("q must be on the pools' device")
     if alibi_slopes is not None and (
             alibi_slopes.dtype is not torch.float32 or alibi_slopes.shape != (n_heads,) or
             alibi_slopes.get_device() != dev or not alibi_slopes.is_contiguous()):
@@ -475,6 +474,14 @@ def _score_mod(q: torch.Tensor, k_pool: torch.Tensor, n_heads: int, softcap: flo
     big = (1 << 31) - 1
     return nat.ScoreMod(softcap, min(window, big), min(sink_tokens, big), _ptr(alibi_slopes),
                         _ptr(prefix_lens), _ptr(first_keys))
+
+
+def _mod_device(k_pool: torch.Tensor, **tensors: torch.Tensor | None) -> None:
+    """A modified-score call's tensors are all on the pools' device."""
+    dev = k_pool.get_device()
+    for name, t in tensors.items():
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{name} must be on the pools' device")
 
 
 def _mod_workspace(n_seqs: int, n_kv_heads: int, rows: int, head_dim: int, device: int,
@@ -551,12 +558,14 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         o_sb, o_st, o_sh = out.stride(0), out.stride(1), out.stride(2)
     if scale is None:
         scale = D ** -0.5
-    mod = _score_mod(q, k_pool, Hq, softcap, alibi_slopes, window, sink_tokens, prefix_lens,
+    mod = _score_mod(q, Hq, softcap, alibi_slopes, window, sink_tokens, prefix_lens,
                      first_keys, B, B)
     if mod is not None and nq > 1 and not causal:
         raise ValueError("modified scores of several query tokens need causal=True")
     if mod is None and causal and nq > 1:
         mod = nat.ScoreMod()
+    if mod is not None:
+        _mod_device(k_pool, q=q, out=out, workspace=workspace)
     if B == 0:
         return out
     dev = _dev_index(q)
@@ -620,10 +629,10 @@ def paged_append_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Ten
         raise ValueError("out must match q's shape with unit last stride")
     if scale is None:
         scale = D ** -0.5
-    mod = _score_mod(q, k_pool, Hq, softcap, alibi_slopes, window, sink_tokens, prefix_lens,
+    mod = _score_mod(q, Hq, softcap, alibi_slopes, window, sink_tokens, prefix_lens,
                      first_keys, B, B)
-    if mod is not None and not (k_new.get_device() == v_new.get_device() == q.get_device()):
-        raise ValueError("k_new and v_new must be on the pools' device")
+    if mod is not None:
+        _mod_device(k_pool, q=q, k_new=k_new, v_new=v_new, out=out, workspace=workspace)
     if B == 0:
         return out
     dev = _dev_index(q)
@@ -685,8 +694,10 @@ def paged_prefill(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         raise ValueError("out must match q's shape with unit last stride")
     if scale is None:
         scale = D ** -0.5
-    mod = _score_mod(q, k_pool, Hq, softcap, alibi_slopes, window, sink_tokens, prefix_lens,
+    mod = _score_mod(q, Hq, softcap, alibi_slopes, window, sink_tokens, prefix_lens,
                      first_keys, B, T)
+    if mod is not None:
+        _mod_device(k_pool, q=q, out=out)
     if B == 0 or T == 0 or max_q_len == 0:
         return out
     dev = _dev_index(q)

@@ -63,8 +63,8 @@ def paged(q: np.ndarray, k_pool: np.ndarray, v_pool: np.ndarray, tables: np.ndar
           scale: float | None = None, first: np.ndarray | None = None,
           prefix: np.ndarray | None = None, **mod) -> tuple[np.ndarray, np.ndarray]:
     """Batched form: sequence b's q_len[b] rows of q (T, Hq, D; uint16 bits of
-    ``dtype``) from row q_start[b] are its last tokens (positions below 0 see
-    nothing); ``first`` per row.  (out, spread) in float64, zeros elsewhere."""
+    ``dtype``) from row q_start[b] are its last tokens (positions below 0 see the
+    prefix alone); ``first`` per row.  (out, spread) in float64, zeros elsewhere."""
     from .rng import to_f32
 
     bs, D = k_pool.shape[2], q.shape[2]

@@ -381,6 +381,55 @@ def test_prefill_last_row_equals_decode(cuda):
     _check(dec, rows)
 
 
+@gpu
+def test_decode_with_every_key_hidden_reads_no_table_entry(cuda):
+    """A token that sees no key needs no valid block: zeros and no error."""
+    q, kp, vp, tables, _ = (t.to(cuda) for t in _host())
+    q += 1
+    vp[:] = float("nan")
+    tables[0] = torch.tensor([-1, 1 << 20])
+    tables[1] = torch.tensor([2, 3])
+    vp[2:] = 0.5
+    ctx = torch.tensor([32, 32], dtype=torch.int32, device=cuda)
+    first = torch.tensor([32, 31], dtype=torch.int32, device=cuda)
+    out = ops.paged_decode(q, kp, vp, tables, ctx, first_keys=first)
+    ops.check_device_errors(0)
+    assert (out[0] == 0).all() and (out[1] == 0.5).all()
+
+
+@gpu
+def test_drafted_tokens_before_the_sequence_see_the_prefix(cuda):
+    """Two cached tokens and four query tokens: those at positions below 0 see
+    the prefix alone, and nothing without one.  Values are exact: V is 1."""
+    q, kp, vp, tables, _ = (t.to(cuda) for t in _host(nq=4))
+    vp[:] = 1
+    ctx = torch.full((2,), 2, dtype=torch.int32, device=cuda)
+    prefix = torch.tensor([1, 0], dtype=torch.int32, device=cuda)
+    out = ops.paged_decode(q, kp, vp, tables, ctx, causal=True, prefix_lens=prefix)
+    ops.check_device_errors(0)
+    assert (out[0] == 1).all() and (out[1, :2] == 0).all() and (out[1, 2:] == 1).all()
+
+
+@gpu
+def test_context_beyond_2_to_30_without_a_window(cuda):
+    """No window hides nothing, however long the context.  All but the first
+    block of the table are one block of zero keys (score 0, value 0); the first
+    block's first key scores 64, so its value 1 has weight 1 / (1 + n e^-64),
+    n = 2^30 + 32, which is 1 to 2e-19 and exact in bf16."""
+    D, bs, blocks = 64, 256, (1 << 22) + 1
+    kp = torch.zeros(2, 1, bs, D, dtype=torch.bfloat16, device=cuda)
+    vp = torch.zeros_like(kp)
+    kp[1, 0, 0], vp[1, 0, 0] = 1, 1
+    q = torch.ones(1, 2, D, dtype=torch.bfloat16, device=cuda)
+    tables = torch.zeros(1, blocks, dtype=torch.int32, device=cuda)
+    tables[0, 0] = 1
+    ctx = torch.tensor([(1 << 30) + 32], dtype=torch.int32, device=cuda)
+    slopes = torch.zeros(2, device=cuda)
+    out = ops.paged_decode(q, kp, vp, tables, ctx, scale=1.0, alibi_slopes=slopes)
+    ops.check_device_errors(0)
+    assert (out == 1).all()
+
+
 # --- refusals -------------------------------------------------------------------------
 
 def _host(B=2, Hq=8, Hkv=2, D=64, nq=None):
@@ -409,6 +458,26 @@ def test_refusals_on_the_host(kw, text):
         ops.paged_append_decode(q, kp, vp, k, k, tables, ctx, **kw)
     with pytest.raises(ValueError, match=text):
         ops.paged_prefill(q, kp, vp, tables, ctx, ctx, ctx, 1, **kw)
+
+
+@gpu
+def test_tensors_off_the_pools_device_are_refused(cuda):
+    on = [t.to(cuda) for t in _host()]
+    q, kp, vp, tables, ctx = on
+    far = torch.empty(q.shape, dtype=q.dtype)
+    k = torch.zeros(2, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="out must be on the pools' device"):
+        ops.paged_decode(*on, window=4, out=far)
+    with pytest.raises(ValueError, match="workspace must be on the pools' device"):
+        ops.paged_decode(*on, window=4, workspace=torch.zeros(1 << 20, dtype=torch.uint8))
+    with pytest.raises(ValueError, match="q must be on the pools' device"):
+        ops.paged_decode(torch.zeros(2, 2, 8, 64, dtype=q.dtype), *on[1:], causal=True)
+    with pytest.raises(ValueError, match="out must be on the pools' device"):
+        ops.paged_append_decode(q, kp, vp, k.to(cuda), k.to(cuda), tables, ctx, window=4, out=far)
+    with pytest.raises(ValueError, match="v_new must be on the pools' device"):
+        ops.paged_append_decode(q, kp, vp, k.to(cuda), k, tables, ctx, window=4)
+    with pytest.raises(ValueError, match="out must be on the pools' device"):
+        ops.paged_prefill(q, kp, vp, tables, ctx, ctx, ctx, 1, window=4, out=far)
 
 
 def test_several_tokens_need_causal():
