@@ -14,6 +14,10 @@
 // D = 128 where rows as M take 16, O^T += V^T.P^T 8 (16 with bf16's low part of P)
 // where they take 16 (32), and Q and O half the registers.  P^T comes from the
 // scores' accumulator layout by an 8 x 8 transpose in the warp (movmatrix).
+// Measured: a capped, windowed step of 64 sequences up to 8192 tokens (32 / 8
+// heads of 128, bf16, 815 MB) 143 us, 5.7 TB/s, 0.88 of the copy rate, 165 us with
+// rows as M; four drafted tokens of 32 sequences (16 rows, 462 MB) 103 us, 4.5
+// TB/s.  Not kept: three blocks an SM for 16 rows (registers spill, 137 us).
 #include <type_traits>
 
 #include "decode_common.cuh"

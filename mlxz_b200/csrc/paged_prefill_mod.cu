@@ -18,8 +18,13 @@
 // store), of which the special-function unit needs 512; two warps of two streams
 // share a scheduler, and two streams without any order between them fill each
 // other's gaps: 4096 new tokens at 16384 with a window of 4096 (32 / 8 heads of
-// 128, bf16) take 357 us, 770 TFLOP/s, against 418 us for one stream of 128-key
-// tiles whose halves meet at every maximum.  Not kept, each right but slower on
+// 128, bf16) take 353 us, 780 TFLOP/s, against 418 us for one stream of 128-key
+// tiles whose halves meet at every maximum (409 us launched back to back, where
+// the power limit lowers the clock).  The tensor core is the next bound: two tiles
+// with P in two bf16 parts take it 2 (8 x 48 + 8 x 64) = 1792 cycles, S at N = 64
+// being held up by its operands' shared memory reads, of the 1970 measured.  A cap
+// of 50 on 512 new tokens at 3584 of eight sequences: 479 us, 538 TFLOP/s; short
+// prompts are bound by an item's latency.  Not kept, each right but slower on
 // that case: P.V issued apart from S, by a second warp (533 us) or by one warp
 // that polls both streams' barriers (425 us with S first, 482 us with P.V first);
 // the MMAs issued by one lane's branch instead of an elected lane (414 us);
