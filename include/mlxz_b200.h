@@ -335,7 +335,10 @@ MZ_API int mz_paged_append_decode_mod(
     uint32_t flags, void *workspace, size_t workspace_bytes, int32_t *dev_err,
     mz_stream_t stream);
 
-/* mz_paged_prefill with modified scores and masks (first_keys per row of q). */
+/* mz_paged_prefill with modified scores and masks (first_keys per row of q).
+ * Where a call has fewer query blocks than SMs, their keys are shared out over
+ * more of them: the order of the sums, and so the last bits of a result, then
+ * depend on n_seqs, max_q_len and max_blocks_per_seq (never on timing). */
 MZ_API int mz_paged_prefill_mod(void *out, int32_t out_dtype, int64_t out_tok_stride,
                                 int64_t out_head_stride, const void *q, int64_t q_tok_stride,
                                 int64_t q_head_stride, int32_t n_rows, const int32_t *q_start,

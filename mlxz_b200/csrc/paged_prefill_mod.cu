@@ -38,6 +38,18 @@
 // tiles of the keys that every row sees (prefix and sinks) and those from its
 // first row's lowest key on; local tile t is tile t or t + skip of the sequence.
 //
+// Few items over long contexts would leave SMs idle: then a cluster of up to eight
+// CTAs takes one item, its 2 to 16 streams a range of the key tiles each, and they
+// join their (m, l, O) through the cluster's shared memory: each stream leaves its
+// O there and writes the joined columns that are its share.  No workspace, no
+// second launch.  With a cap of 50, 32 tokens at 16384 take 44 us (338 us as whole
+// items), 64 at 2000 22 us (51), 32 at 600 19 us (22); 64 behind a window of 4096
+// 25 us (73).  Joining costs 3 to 5 us, so a part has two tiles at least: parts of
+// four made 32 tokens at 600 22 us and 1 at 400 17 instead of 14 us.  Not kept: the
+// odd last item of a CTA among many shared by its two streams in the same way
+// (window 350 against 360 us, but documents 112 against 105, a cap on 256 items of
+// 8192 keys 252 against 232: a stream alone runs faster than one of two).
+//
 // Every wait is bounded; one that gives up sets MZ_DEVERR_TIMEOUT and the abort
 // flag, every role leaves its loop, the issuing warps wait (bounded) for their
 // copies and MMAs in flight, and the TMEM is freed.
@@ -55,6 +67,7 @@ constexpr int kN = 64;       // keys per tile
 constexpr int kSlots = 2;    // K slots, V slots and S buffers of a stream
 constexpr int kStreams = 2;
 constexpr int kSoftWarps = 4;  // per stream
+constexpr int kPartTiles = 2;  // tiles of a split item's part at least
 constexpr int kThreads = 32 * kStreams * (kSoftWarps + 2);
 constexpr uint32_t kTmemCols = 512;
 constexpr float kRescaleLog2 = 8.f;
@@ -69,6 +82,9 @@ struct Cfg {
   static constexpr int kQ = (D / 64) * kM * 128;  // 128 rows x D, chunk-major
   static constexpr int kStream = kQ + 2 * kSlots * kTile;
   static constexpr int kBar = kStreams * kStream;
+  // a split item's O (fp32, column by column) in place of Q and K, (m, l) behind it
+  static constexpr int kMl = kQ + kSlots * kTile;
+  static_assert(kMl == kM * D * 4, "O takes the place of Q and the K slots");
   static constexpr int kSmemBytes = kBar + 256 + 1024;
 };
 
@@ -83,7 +99,18 @@ struct Item {
   // row's other keys start below it; head_tiles, skip: tiles of the head, tiles
   // left out behind them
   int prefix, head, lo, head_tiles, skip;
-  __device__ __forceinline__ int own(int t) const { return t < head_tiles ? t : t + skip; }
+  int t0;  // first tile of this part, in a split item
+  template <bool SPLIT>
+  __device__ __forceinline__ int own(int t) const {
+    if constexpr (SPLIT) t += t0;
+    return t < head_tiles ? t : t + skip;
+  }
+  // Part i of n, which may be empty.
+  __device__ __forceinline__ void cut(int i, int n) {
+    const int per = (ntiles + n - 1) / n;
+    t0 = min(i * per, ntiles);
+    ntiles = min(per, ntiles - t0);
+  }
 };
 
 // Where a stream's search for its next item stands: sequence b's first item is
@@ -156,6 +183,7 @@ __device__ __forceinline__ bool item_at(const PParams &p, Walk &w, int e, Item &
   // the tile of lo, or the last causal one, is read in any case
   it.skip = max(0, min(it.lo, last) / kN - it.head_tiles);
   it.ntiles = (it.kv_len + kN - 1) / kN - it.skip;
+  it.t0 = 0;
   return true;
 }
 
@@ -176,9 +204,96 @@ __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t phase,
   }
 }
 
+__device__ __forceinline__ int cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return static_cast<int>(r);
+}
+__device__ __forceinline__ int cluster_size() {
+  uint32_t n;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+  return static_cast<int>(n);
+}
+// All threads of the cluster; what was written before it is seen after it.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile(
+      "barrier.cluster.arrive.release;\n\t"
+      "barrier.cluster.wait.acquire;" ::: "memory");
+}
+// Shared memory of the cluster's CTA `rank`, at this CTA's address `at`.
+__device__ __forceinline__ uint32_t peer_smem(uint32_t at, int rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(at), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ float ld_peer(uint32_t at) {
+  float x;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(at) : "memory");
+  return x;
+}
+__device__ __forceinline__ float2 ld_peer2(uint32_t at) {
+  float2 x;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x.x), "=f"(x.y) : "r"(at) : "memory");
+  return x;
+}
+
+// Columns [part, part + 1) * D / N of a split item's row, joined from its N parts
+// (part j: stream j & 1 of rank j >> 1, at the same place in every CTA; `cta`:
+// stream 0's memory here) and written to out at `ob`.
+template <int D, bool BF16, int N>
+__device__ __forceinline__ void join_parts(const PParams &p, uint32_t cta, int row, int part,
+                                           int64_t ob) {
+  using C = Cfg<D>;
+  constexpr int kCols = D / N, kStep = N < 8 ? 32 / N : 4;  // 32 loads in flight, or more
+  static_assert(kCols % kStep == 0, "whole steps");
+  uint32_t from[N];
+  float2 ml[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    from[j] = peer_smem(cta + (j & 1) * C::kStream, j >> 1);
+    ml[j] = ld_peer2(from[j] + C::kMl + 8 * row);
+  }
+  // weights of the parts; none for those without a key of the row, or any tile
+  float w[N], top = kNoMax, sum = 0.f;
+#pragma unroll
+  for (int j = 0; j < N; ++j) top = ml[j].y != 0.f ? fmaxf(top, ml[j].x) : top;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    w[j] = ml[j].y != 0.f ? fast_exp2(ml[j].x - top) : 0.f;
+    sum = fmaf(w[j], ml[j].y, sum);
+  }
+  const float inv = decode::row_inverse(sum);
+#pragma unroll 1
+  for (int c = part * kCols; c < (part + 1) * kCols; c += kStep) {
+    float x[N][kStep], acc[kStep];
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+#pragma unroll
+      for (int i = 0; i < kStep; ++i) x[j][i] = ld_peer(from[j] + 4 * ((c + i) * kM + row));
+#pragma unroll
+    for (int i = 0; i < kStep; ++i) {
+      acc[i] = 0.f;
+      // (a part of no weight may have left nothing there)
+#pragma unroll
+      for (int j = 0; j < N; ++j) acc[i] = w[j] != 0.f ? fmaf(w[j], x[j][i], acc[i]) : acc[i];
+      acc[i] *= inv;
+    }
+#pragma unroll
+    for (int i = 0; i < kStep; i += 4) {
+      if (p.out_f32)
+        *reinterpret_cast<float4 *>(static_cast<float *>(p.out) + ob + c + i) =
+            make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]);
+      else
+        *reinterpret_cast<uint2 *>(static_cast<uint16_t *>(p.out) + ob + c + i) = make_uint2(
+            pack2<BF16>(acc[i], acc[i + 1]), pack2<BF16>(acc[i + 2], acc[i + 3]));
+    }
+  }
+}
+
 // MODE 1: masks; 2: masks and the bias by distance; 3: these and capped scores.
 // From 2 on the scores take their final form, in log2 units, in registers.
-template <int D, bool BF16, int MODE>
+// SPLIT: the cluster's streams share one item, item (block / cluster size).
+template <int D, bool BF16, int MODE, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_prefill_mod_kernel(const __grid_constant__ CUtensorMap tmK,
                              const __grid_constant__ CUtensorMap tmV, const PParams p) {
@@ -219,10 +334,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // Items go to the streams in turn, all first streams before all second ones:
   // in the last round they spread over the SMs.
-  const int e0 = st * gridDim.x + blockIdx.x, e_step = kStreams * gridDim.x;
+  const int ranks = SPLIT ? cluster_size() : 1;
+  const int e0 = SPLIT ? blockIdx.x / ranks : st * gridDim.x + blockIdx.x;
+  const int e_step = kStreams * gridDim.x;
   Walk walk;
   auto next_item = [&](int &e, Item &it) {
     for (bool end = false;; e += e_step) {
+      if (SPLIT && e != e0) return false;
       if (item_at(p, walk, e, it, &end)) return true;
       if (end) return false;
     }
@@ -248,6 +366,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   int g = 0;  // tiles of this stream so far: slot g % 2, barrier phase g / 2
   int e = e0;
   bool have = next_item(e, it), ok = true;
+  const bool found = have;
+  const int parts = kStreams * ranks, part = SPLIT ? kStreams * cluster_rank() + st : 0;
+  if (SPLIT && have) {
+    it.cut(part, parts);
+    have = it.ntiles > 0;
+  }
+  float m_part = kNoMax, l_part = 0.f;  // a split item's
 
   if (copies) {
     // ---------------- copies: K of tile t, then V of tile t - 1 ----------------
@@ -259,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // lane l holds box l % nst of tile per * x + l / nst; block ids are loaded
       // one such set ahead of their use
       auto box_key = [&](int x) {
-        return it.own(per * x + (lane >> nst_log2)) * kN + (lane & (nst - 1)) * sub;
+        return it.template own<SPLIT>(per * x + (lane >> nst_log2)) * kN + (lane & (nst - 1)) * sub;
       };
       auto ids = [&](int x) -> int32_t {
         const int t = box_key(x);
@@ -276,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         return static_cast<int>(((int64_t)blk * p.Hkv + it.h) * p.bs + t % p.bs);
       };
       auto load = [&](const CUtensorMap *tm, uint32_t dst, uint32_t fbar, int t, int y) {
-        const int nsub = min(nst, (it.kv_len - it.own(t) * kN + sub - 1) >> p.sub_log2);
+        const int nsub = min(nst, (it.kv_len - it.template own<SPLIT>(t) * kN + sub - 1) >> p.sub_log2);
         if (lane == 0)
           mbar_arrive_expect_tx(fbar, static_cast<uint32_t>(nsub * sub * D * 2));
         __syncwarp();
@@ -417,7 +542,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int e2 = e + e_step;
       bool have2 = false;
       for (int i = 0; i < it.ntiles; ++i) {
-        const int j = g + i, s = j & 1, tile = it.own(i);
+        const int j = g + i, s = j & 1, tile = it.template own<SPLIT>(i);
         if (!wait(kBarSFull + s, j >> 1)) {
           ok = false;
           break;
@@ -639,6 +764,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         break;
       }
       tc::fence_after_sync();
+      if constexpr (SPLIT) {
+        m_part = m_used;
+        l_part = l;
+        break;
+      }
       const float inv = decode::row_inverse(l);
       const int64_t ob = (int64_t)(p.q_start[it.b] + tok) * p.o_st + (int64_t)hq * p.o_sh;
 #pragma unroll
@@ -679,6 +809,40 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   }
 
+  if constexpr (SPLIT) {
+    // Every role comes here, also one that gave up: the barriers end.
+    const int row = threadIdx.x & (kM - 1);
+    if (warp < 8 && found && ok) {
+      if (have) {
+        // this stream's copies and products are all complete: O takes the place
+        // of its Q and K, neighbouring rows side by side
+        float *o = reinterpret_cast<float *>(smem + st * C::kStream) + row;
+        const uint32_t o_col = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + 128 * st;
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          uint32_t r[32];
+          tc::ld32(o_col + 32 * c, r);
+          tc::wait_ld();
+#pragma unroll
+          for (int x = 0; x < 32; ++x) o[(32 * c + x) * kM] = __uint_as_float(r[x]);
+        }
+      }
+      *reinterpret_cast<float2 *>(smem + st * C::kStream + C::kMl + 8 * row) =
+          make_float2(m_part, l_part);
+    }
+    cluster_sync();
+    if (warp < 8 && found && ok && it.q0 + row / p.G < it.q_hi) {
+      const int64_t ob = (int64_t)(p.q_start[it.b] + it.q0 + row / p.G) * p.o_st +
+                         (int64_t)(it.h * p.G + row % p.G) * p.o_sh;
+      const uint32_t cta = sbase - st * C::kStream;  // stream 0
+      if (parts == 2) join_parts<D, BF16, 2>(p, cta, row, part, ob);
+      else if (parts == 4) join_parts<D, BF16, 4>(p, cta, row, part, ob);
+      else if (parts == 8) join_parts<D, BF16, 8>(p, cta, row, part, ob);
+      else join_parts<D, BF16, 16>(p, cta, row, part, ob);
+    }
+    cluster_sync();  // no CTA leaves while another one reads from it
+  }
+
   tc::fence_before_sync();
   __syncthreads();
   if (warp == 9) {
@@ -687,11 +851,72 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-template <int D, bool BF16, int MODE>
+template <int D, bool BF16, int MODE, bool SPLIT>
 int smem_attr() {
   static DeviceOnce once;
-  return smem_optin(paged_prefill_mod_kernel<D, BF16, MODE>, Cfg<D>::kSmemBytes, once,
+  return smem_optin(paged_prefill_mod_kernel<D, BF16, MODE, SPLIT>, Cfg<D>::kSmemBytes, once,
                     "mz_paged_prefill_mod: shared memory attribute");
+}
+
+inline cudaLaunchAttribute cluster_of(int x) {
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = x;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  return at;
+}
+
+// Clusters of X CTAs that fit the device at once (0: none).
+template <int D, bool BF16, int MODE, int X>
+int max_clusters(int *n) {
+  static DeviceOnce once;
+  return device_once(
+      once,
+      [](int *value) {
+        cudaLaunchAttribute at = cluster_of(X);
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(X);
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = Cfg<D>::kSmemBytes;
+        cfg.attrs = &at;
+        cfg.numAttrs = 1;
+        return cudaOccupancyMaxActiveClusters(
+            value, paged_prefill_mod_kernel<D, BF16, MODE, true>, &cfg);
+      },
+      n, "mz_paged_prefill_mod: cluster occupancy");
+}
+
+// `items` (sequence, head, query block) at most, of up to `tiles` key tiles.
+template <int D, bool BF16, int MODE>
+int launch(const CUtensorMap &tk, const CUtensorMap &tv, const PParams &p, int64_t items,
+           int64_t tiles, int sms, cudaStream_t s) {
+  // One item per cluster where all items fit the device at once, in the largest
+  // clusters whose streams get kPartTiles tiles each; else whole items.
+  int x = 0;
+  if (items <= sms && tiles >= kStreams * kPartTiles) {
+    if (int rc = smem_attr<D, BF16, MODE, true>()) return rc;
+    int n2 = 0, n4 = 0, n8 = 0;
+    if (int rc = max_clusters<D, BF16, MODE, 2>(&n2)) return rc;
+    if (int rc = max_clusters<D, BF16, MODE, 4>(&n4)) return rc;
+    if (int rc = max_clusters<D, BF16, MODE, 8>(&n8)) return rc;
+    auto fits = [&](int n, int y) { return items <= n && tiles >= (int64_t)y * kStreams * kPartTiles; };
+    x = fits(n8, 8) ? 8 : fits(n4, 4) ? 4 : fits(n2, 2) ? 2 : 1;
+  } else if (int rc = smem_attr<D, BF16, MODE, false>()) {
+    return rc;
+  }
+  cudaLaunchAttribute at = cluster_of(x);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(x ? items * x : std::min<int64_t>(items, sms)));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Cfg<D>::kSmemBytes;
+  cfg.stream = s;
+  cfg.attrs = &at;
+  cfg.numAttrs = x > 1 ? 1 : 0;
+  const cudaError_t e =
+      x ? cudaLaunchKernelEx(&cfg, paged_prefill_mod_kernel<D, BF16, MODE, true>, tk, tv, p)
+        : cudaLaunchKernelEx(&cfg, paged_prefill_mod_kernel<D, BF16, MODE, false>, tk, tv, p);
+  if (e != cudaSuccess) return cuda_fail(e, "mz_paged_prefill_mod");
+  return MZ_OK;
 }
 
 }  // namespace two
@@ -728,29 +953,26 @@ extern "C" int mz_paged_prefill_mod(void *out, int32_t out_dtype, int64_t out_to
   if (sms <= 0) return fail(MZ_ERR_CUDA, "%s: cannot query the SM count", fn);
   if (items + two::kStreams * (int64_t)sms >= (int64_t(1) << 31))
     return fail(MZ_ERR_UNSUPPORTED, "%s: too many query blocks", fn);
-  const dim3 grid(static_cast<unsigned>(std::min<int64_t>(items, sms)));
+  // key tiles of an item at most: of its table, or of what a window leaves
+  const int tpc = kM / p.G;
+  int64_t tiles = ((int64_t)max_blocks_per_seq * block_size + two::kN - 1) / two::kN;
+  if (p.mod.window > 0 && !p.mod.prefix)
+    tiles = std::min(tiles, ((int64_t)p.mod.window + tpc) / two::kN + 2 + p.mod.sink / two::kN);
   const bool bf16 = dtype == MZ_DTYPE_BF16;
   const int mode = p.mod.z_scale != 0.f ? 3 : p.mod.slopes ? 2 : 1;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-#define MZ_TWO(D_, BF_, MODE_)                                                       \
-  do {                                                                               \
-    if (int rc = two::smem_attr<D_, BF_, MODE_>()) return rc;                        \
-    two::paged_prefill_mod_kernel<D_, BF_, MODE_>                                    \
-        <<<grid, two::kThreads, two::Cfg<D_>::kSmemBytes, s>>>(tk, tv, p);           \
-  } while (0)
-#define MZ_TWO_MODE(D_, BF_)                                                         \
-  do {                                                                               \
-    if (mode == 1) MZ_TWO(D_, BF_, 1);                                               \
-    else if (mode == 2) MZ_TWO(D_, BF_, 2);                                          \
-    else MZ_TWO(D_, BF_, 3);                                                         \
-  } while (0)
+  int rc = MZ_OK;
+#define MZ_TWO(D_, BF_)                                                              \
+  rc = mode == 1   ? two::launch<D_, BF_, 1>(tk, tv, p, items, tiles, sms, s)        \
+       : mode == 2 ? two::launch<D_, BF_, 2>(tk, tv, p, items, tiles, sms, s)        \
+                   : two::launch<D_, BF_, 3>(tk, tv, p, items, tiles, sms, s)
   if (head_dim == 128) {
-    if (bf16) MZ_TWO_MODE(128, true); else MZ_TWO_MODE(128, false);
+    if (bf16) MZ_TWO(128, true); else MZ_TWO(128, false);
   } else {
-    if (bf16) MZ_TWO_MODE(64, true); else MZ_TWO_MODE(64, false);
+    if (bf16) MZ_TWO(64, true); else MZ_TWO(64, false);
   }
-#undef MZ_TWO_MODE
 #undef MZ_TWO
+  if (rc) return rc;
   MZ_CHECK_LAUNCH(fn);
   return MZ_OK;
 }

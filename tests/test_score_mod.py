@@ -365,6 +365,106 @@ def test_prefill_hidden_blocks_may_be_anything(cuda, fill):
     assert torch.equal(got, want)
 
 
+# Few query blocks over long tables: their keys are shared out over clusters of 8, 4,
+# 2 and 1 blocks, or (many query blocks, or short tables) not at all.
+FEW = [
+    ("bf16", 128, 4, 16, 2, [4500], [5]),
+    ("f16", 64, 8, 32, 1, [4490, 4100, 70], [1, 20, 16]),
+    ("f16", 128, 2, 16, 2, [2100, 300, 40], [70, 64, 0]),
+    ("bf16", 64, 4, 64, 3, [1100, 65, 1], [33, 65, 1]),
+    ("bf16", 128, 16, 16, 5, [600, 590, 513], [30, 1, 9]),
+    ("bf16", 64, 4, 16, 8, [650] * 6 + [70] * 4, [40] * 9 + [0]),
+]
+
+
+@gpu
+@pytest.mark.parametrize("mod", ["cap", "slopes", "window_sinks", "docs", "prefix", "all"])
+@pytest.mark.parametrize("dtype,D,G,bs,Hkv,ctx,qlen", FEW)
+def test_prefill_of_few_rows(cuda, mod, dtype, D, G, bs, Hkv, ctx, qlen):
+    case = _prefill_case(60 + D + G, ctx, qlen, dtype, D, G, bs, Hkv)
+    kw, ow = _mod_args(MODS[mod], Hkv * G, ctx, qlen, True, cuda)
+    for out_dtype in (torch.float32, TORCH[dtype]):
+        out = _prefill(case, dtype, cuda, kw, out_dtype)
+        _check(out, osm.paged(case["qp"], case["kp"], case["vp"], case["tables"],
+                              case["q_start"], case["q_len"], case["ctx"], dtype, **ow), mod)
+
+
+@gpu
+@pytest.mark.parametrize("fill", [float("nan"), float("inf")])
+def test_prefill_of_few_rows_with_hidden_blocks_and_empty_rows(cuda, fill):
+    """A window over part of the keys, whose other blocks may be anything; rows
+    that see nothing; rows behind the last sequence."""
+    ctx, qlen, window, sink = [5000, 3100], [40, 9], 3000, 20
+    case = _prefill_case(61, ctx, qlen, "bf16", 128, 4, 16, 1)
+    case["qp"] = rng.normal(61, (60, 4, 128), "bf16", stream=9)
+    first = np.zeros(60, dtype=np.int32)
+    first[3:36] = 1 << 30  # but for the sinks; the second query block sees more
+    kp, vp, tables, c = _dev(case, "bf16", cuda)
+    for b, (n, m) in enumerate(zip(ctx, qlen)):
+        lo = n - m - window + 1
+        for t in range(sink, lo):
+            blk = int(tables[b, t // 16])
+            kp[blk, :, t % 16] = fill
+            vp[blk, :, t % 16] = fill
+        for j in range(-(-sink // 16), lo // 16):
+            tables[b, j] = -1
+    for s in (sink, 0):
+        if s == 0:
+            kp[tables[:, 0].long()] = fill
+            kp[tables[:, 1].long()] = fill
+        out = torch.full((60, 4, 128), 7.0, dtype=torch.bfloat16, device=cuda)
+        _prefill(case, "bf16", cuda, dict(window=window, sink_tokens=s,
+                                          first_keys=torch.from_numpy(first).to(cuda)),
+                 out=out, pools=(kp, vp, tables, c))
+        assert (out[49:] == 7).all() and (s > 0 or not out[3:36].any())
+        want = osm.paged(case["qp"], case["kp"], case["vp"], case["tables"], case["q_start"],
+                         case["q_len"], case["ctx"], "bf16", first=first, window=window, sink=s)
+        _check(out[:49], (want[0][:49], want[1][:49]))
+
+
+@gpu
+def test_prefill_of_few_rows_in_a_graph_and_with_a_bad_sequence(cuda):
+    """Lengths that change between replays, one stream next to another; a
+    sequence in error leaves its rows and the others' results alone."""
+    ctx, qlen = [4300, 4300], [6, 4]
+    case = _prefill_case(62, ctx, qlen, "f16", 128, 4, 16, 2)
+    kp, vp, tables, c = _dev(case, "f16", cuda)
+    i = {k: torch.from_numpy(case[k]).to(cuda) for k in ("q_start", "q_len")}
+    q = to_dev(case["qp"], "f16", cuda)
+    kw = dict(softcap=25.0, first_keys=torch.full((10,), 3, dtype=torch.int32, device=cuda))
+    runs = []
+    for _ in range(2):
+        s, g = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            call = lambda: ops.paged_prefill(q, kp, vp, tables, i["q_start"], i["q_len"], c, 6, **kw)
+            call()
+            with torch.cuda.graph(g, stream=s):
+                runs.append((g, s, call()))
+    torch.cuda.synchronize()
+    for lens in ([4300, 4300], [6, 4], [200, 4001]):
+        c.copy_(torch.tensor(lens, dtype=torch.int32))
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for g, s, _ in runs:
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        ops.check_device_errors(0)
+        want = osm.paged(case["qp"], case["kp"], case["vp"], case["tables"], case["q_start"],
+                         case["q_len"], np.array(lens), "f16", softcap=25.0,
+                         first=np.full(10, 3))
+        for _, _, out in runs:
+            _check(out, want, lens)
+    c.copy_(torch.tensor([2, 4001], dtype=torch.int32))  # fewer tokens than query rows
+    out = torch.full_like(runs[0][2], 7.0)
+    ops.paged_prefill(q, kp, vp, tables, i["q_start"], i["q_len"], c, 6, out=out, **kw)
+    with pytest.raises(DeviceError, match="context length"):
+        ops.check_device_errors(0)
+    assert (out[:6] == 7).all()
+    _check(out[6:], (want[0][6:], want[1][6:]))
+
+
 @gpu
 def test_prefill_last_row_equals_decode(cuda):
     case = _prefill_case(54, [700, 250], [64, 9], "f16", 128, 8, 16, 1)
