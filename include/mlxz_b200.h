@@ -617,6 +617,26 @@ MZ_API int mz_paged_decode_q(void *out, int32_t out_dtype, int64_t out_seq_strid
                              void *workspace, size_t workspace_bytes, int32_t *dev_err,
                              mz_stream_t stream);
 
+/* ------------------------------------------------------------------------ */
+/* Entry points by number.                                                   */
+/* ------------------------------------------------------------------------ */
+
+enum mz_packed_op {
+  MZ_OP_PAGED_PLAN = 0,
+  MZ_OP_QK_NORM_ROPE = 1,
+  MZ_OP_PAGED_DECODE_MOD = 2,
+  MZ_OP_PAGED_APPEND_DECODE_MOD = 3,
+  MZ_OP_PAGED_PREFILL_MOD = 4
+};
+
+/* Calls the entry point `op` (enum mz_packed_op) with its arguments, in order,
+ * in n_slots slots of 8 bytes: integers as int64, pointers as their address,
+ * floats as double.  Same work, checks and status as the call itself; for
+ * callers whose foreign function interface pays per argument.  Integers outside
+ * their argument's type, and another number of slots than the entry point has
+ * arguments, are refused (MZ_ERR_INVALID_ARG). */
+MZ_API int mz_call_packed(int32_t op, const void *slots, int32_t n_slots);
+
 #ifdef __cplusplus
 }
 #endif

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from pathlib import Path
 
@@ -163,7 +164,15 @@ _SIGNATURES: dict[str, list] = {
                           _i32, _i32, _f32, _i32, _i32, _vp, _sz, _vp, _vp],
     "mz_block_pack": [_vp, _vp, _i64, _i32, _i64, _vp, _i32, _i64, _vp, _vp],
     "mz_block_unpack": [_vp, _i64, _i32, _i64, _vp, _vp, _i32, _i64, _vp, _vp],
+    "mz_call_packed": [_i32, ctypes.c_char_p, _i32],
 }
+
+# name -> (number for mz_call_packed, packer of its arguments, how many)
+_PACKED = {name: (op, struct.Struct("=" + "".join("d" if t is _f32 else "q"
+                                                  for t in _SIGNATURES[name])).pack,
+                  len(_SIGNATURES[name]))
+           for op, name in enumerate(("mz_paged_plan", "mz_qk_norm_rope", "mz_paged_decode_mod",
+                                      "mz_paged_append_decode_mod", "mz_paged_prefill_mod"))}
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
@@ -220,3 +229,12 @@ def check(status: int) -> None:
 
 def call(name: str, *args) -> None:
     check(getattr(lib(), name)(*args))
+
+
+def call_packed(name: str, *args) -> None:
+    """``call`` for the entry points of mz_call_packed, with pointers as plain
+    addresses (0 for none): one conversion instead of one per argument."""
+    op, pack, n = _PACKED[name]
+    status = lib().mz_call_packed(op, pack(*args), n)
+    if status:
+        check(status)

@@ -103,16 +103,20 @@ def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+def _at(t: torch.Tensor | None) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
 def _call(device: int, name: str, *args) -> None:
-    """nat.call with the error word and the current stream behind ``args``, and
+    """nat.call_packed with the error word and the current stream behind ``args``, and
     ``device`` current: a launch goes to the current device, which need not be
     the tensors' own."""
     err = error_word(device).data_ptr()
     if torch._C._cuda_getDevice() == device:
-        nat.call(name, *args, err, torch._C._cuda_getCurrentRawStream(device))
+        nat.call_packed(name, *args, err, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
-            nat.call(name, *args, err, _stream(device))
+            nat.call_packed(name, *args, err, _stream(device))
     if _DEBUG:
         check_device_errors(device)
 
@@ -287,7 +291,7 @@ def paged_plan(block_tables: torch.Tensor, ctx_lens: torch.Tensor, q_lens: torch
         n_rows + 3 * B + 1).split_with_sizes((n_rows, B, B, B, 1))
     slots = block_tables.new_empty(n_rows, dtype=torch.int64)
     _call(dev, "mz_paged_plan", block_tables.data_ptr(), max(width, 1), ctx_lens.data_ptr(),
-          q_lens.data_ptr(), _ptr(held), _ptr(new_ids), 0 if new_ids is None else new_ids.numel(),
+          q_lens.data_ptr(), _at(held), _at(new_ids), 0 if new_ids is None else new_ids.numel(),
           B, n_rows, block_size, n_blocks, q_start.data_ptr(), positions.data_ptr(),
           slots.data_ptr(), lengths.data_ptr(), held_out.data_ptr(), n_new.data_ptr())
     return PagedPlan(q_start, positions, slots, lengths, held_out, n_new)
@@ -331,25 +335,21 @@ def _rope_args(q, positions, inv_freq, q_weight, k_weight, eps, weight_offset, i
         if x.dtype is not w_dtype or x.shape != (D,) or x.get_device() != dev or \
                 not x.is_contiguous():
             raise ValueError(f"norm weights must be contiguous [{D}] of one dtype on {q.device}")
-    return (positions.data_ptr(), T, n_axes, inv_freq.data_ptr(), _ptr(freq_axes), 2 * half,
-            1 if interleaved else 0, _ptr(q_weight), _ptr(k_weight),
+    return (positions.data_ptr(), T, n_axes, inv_freq.data_ptr(), _at(freq_axes), 2 * half,
+            1 if interleaved else 0, _at(q_weight), _at(k_weight),
             0 if w_dtype is None else dtype_code(w_dtype), weight_offset,
             0.0 if eps is None else eps, 0 if eps is None else 1)
 
 
-def _heads(t: torch.Tensor, name: str, like: torch.Tensor, n_heads: int | None = None
-           ) -> tuple[int, int, int]:
-    """(pointer, token stride, head stride) of a tensor ``[T, heads, D]`` like
-    ``like`` in all but the heads."""
-    shape, want = t.shape, like.shape
-    if len(shape) == 3 and shape[0] == want[0] and shape[2] == want[2] and \
-            t.dtype is like.dtype and t.get_device() == like.get_device() and \
-            (n_heads is None or shape[1] == n_heads):
+def _heads(t: torch.Tensor, name: str, T: int, n_heads: int, like: torch.Tensor,
+           dtype: torch.dtype, dev: int) -> tuple[int, int, int]:
+    """(pointer, token stride, head stride) of a tensor ``[T, n_heads, D]`` of
+    the last dimension, dtype and device of ``like``."""
+    if t.shape == (T, n_heads, like.shape[-1]) and t.dtype is dtype and t.get_device() == dev:
         ts, hs, one = t.stride()
         if one == 1:
             return t.data_ptr(), ts, hs
-    heads = "heads" if n_heads is None else f"{n_heads} heads"
-    raise ValueError(f"{name} must be [{want[0]}, {heads}, {want[2]}] of {like.dtype} on "
+    raise ValueError(f"{name} must be [{T}, {n_heads} heads, {like.shape[-1]}] of {dtype} on "
                      f"{like.device} with unit last stride")
 
 
@@ -371,18 +371,19 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
     is.  ``q_out`` / ``k_out`` may be q / k themselves."""
     if q.dim() != 3:
         raise ValueError("q must be [T, heads, D] with unit last stride")
-    q_at, k_at = _heads(q, "q", q), _heads(k, "k", q)
+    T, Hq, D = q.shape
+    Hkv = k.shape[1] if k.dim() == 3 else 0
+    of = q, q.dtype, q.get_device()
+    q_at, k_at = _heads(q, "q", T, Hq, *of), _heads(k, "k", T, Hkv, *of)
     args = _rope_args(q, positions, inv_freq, q_weight, k_weight, eps, weight_offset, interleaved,
                       freq_axes)
     if q_out is None:
         q_out = q.new_empty(q.shape)
     if k_out is None:
         k_out = k.new_empty(k.shape)
-    T, Hq, D = q.shape
-    Hkv = k.shape[1]
-    qo_at, ko_at = _heads(q_out, "q_out", q, Hq), _heads(k_out, "k_out", q, Hkv)
+    qo_at, ko_at = _heads(q_out, "q_out", T, Hq, *of), _heads(k_out, "k_out", T, Hkv, *of)
     _call(_dev_index(q), "mz_qk_norm_rope", *qo_at, *ko_at, *q_at, *k_at,
-          None, 0, 0, None, None, None, 0, 0, *args, T, Hq, Hkv, D, dtype_code(q.dtype))
+          0, 0, 0, 0, 0, 0, 0, 0, *args, T, Hq, Hkv, D, dtype_code(q.dtype))
     return q_out, k_out
 
 
@@ -402,8 +403,9 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     if q.dim() != 3 or q.shape[2] != D or q.dtype is not k_pool.dtype or \
             q.get_device() != k_pool.get_device():
         raise ValueError(f"q must be [T, heads, {D}] of the pools' dtype and device")
-    q_at, k_at, v_at = _heads(q, "q", q), _heads(k, "k", q, H), _heads(v, "v", q, H)
     T, Hq, _ = q.shape
+    of = q, q.dtype, q.get_device()
+    q_at, k_at, v_at = _heads(q, "q", T, Hq, *of), _heads(k, "k", T, H, *of), _heads(v, "v", T, H, *of)
     if slot_mapping.dtype is not torch.int64 or slot_mapping.numel() != T or \
             slot_mapping.get_device() != q.get_device() or not slot_mapping.is_contiguous():
         raise ValueError("slot_mapping must be a contiguous int64 [T] on the pool device")
@@ -411,8 +413,8 @@ def qk_norm_rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                       freq_axes)
     if q_out is None:
         q_out = q.new_empty(q.shape)
-    qo_at = _heads(q_out, "q_out", q, Hq)
-    _call(_dev_index(q), "mz_qk_norm_rope", *qo_at, None, 0, 0, *q_at, *k_at,
+    qo_at = _heads(q_out, "q_out", T, Hq, *of)
+    _call(_dev_index(q), "mz_qk_norm_rope", *qo_at, 0, 0, 0, *q_at, *k_at,
           *v_at, k_pool.data_ptr(), v_pool.data_ptr(), slot_mapping.data_ptr(), bs, n_blocks,
           *args, T, Hq, H, D, dtype_code(q.dtype))
     return q_out
@@ -577,7 +579,7 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
         _call(dev, "mz_paged_decode_mod", out.data_ptr(), dtype_code(out_dtype), o_sb, o_st, o_sh,
               q.data_ptr(), q_sb, q_st, q_sh, nq, k_pool.data_ptr(), v_pool.data_ptr(),
               block_tables.data_ptr(), block_tables.shape[1], ctx_lens.data_ptr(), B, Hq, Hkv, D,
-              bs, n_blocks, float(scale), ctypes.byref(mod), dtype_code(q.dtype), num_warps,
+              bs, n_blocks, float(scale), ctypes.addressof(mod), dtype_code(q.dtype), num_warps,
               workspace.data_ptr(), workspace.numel())
         return out
     nat.call("mz_paged_decode", out.data_ptr(), dtype_code(out_dtype), o_sb, o_st, o_sh,
@@ -645,7 +647,7 @@ def paged_append_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Ten
               out.stride(0), out.stride(1), q.data_ptr(), q.stride(0), q.stride(1),
               k_pool.data_ptr(), v_pool.data_ptr(), k_new.data_ptr(), v_new.data_ptr(),
               k_new.stride(0), k_new.stride(1), block_tables.data_ptr(), block_tables.shape[1],
-              ctx_lens.data_ptr(), B, Hq, Hkv, D, bs, n_blocks, float(scale), ctypes.byref(mod),
+              ctx_lens.data_ptr(), B, Hq, Hkv, D, bs, n_blocks, float(scale), ctypes.addressof(mod),
               dtype_code(q.dtype), num_warps,
               (nat.MZ_LAUNCH_OVERLAP_PREVIOUS if overlap_previous else 0)
               | (nat.MZ_DECODE_BATCH_INVARIANT if batch_invariant else 0),
@@ -706,7 +708,7 @@ def paged_prefill(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
               out.stride(1), q.data_ptr(), q.stride(0), q.stride(1), T, q_start.data_ptr(),
               q_len.data_ptr(), int(max_q_len), k_pool.data_ptr(), v_pool.data_ptr(),
               block_tables.data_ptr(), block_tables.shape[1], ctx_lens.data_ptr(), B, Hq, Hkv, D,
-              bs, n_blocks, float(scale), ctypes.byref(mod), dtype_code(q.dtype))
+              bs, n_blocks, float(scale), ctypes.addressof(mod), dtype_code(q.dtype))
         return out
     nat.call("mz_paged_prefill", out.data_ptr(), dtype_code(out_dtype), out.stride(0),
              out.stride(1), q.data_ptr(), q.stride(0), q.stride(1), T, q_start.data_ptr(),

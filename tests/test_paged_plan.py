@@ -228,3 +228,42 @@ def test_plan_c_abi_argument_errors():
         assert call(**kw) == _native.MZ_ERR_INVALID_ARG, kw
     assert call(width=1 << 28, bs=16) == _native.MZ_ERR_UNSUPPORTED
     assert call(width=1 << 20, B=1 << 12) == _native.MZ_ERR_UNSUPPORTED
+
+
+# --- entry points by number ----------------------------------------------------------------
+
+def test_packed_calls_refuse_what_is_no_call():
+    lib = _native.lib()
+    slots = bytes(8 * 64)
+    assert lib.mz_call_packed(99, slots, 19) == _native.MZ_ERR_INVALID_ARG
+    assert lib.mz_call_packed(-1, slots, 19) == _native.MZ_ERR_INVALID_ARG
+    assert "no entry point" in _native.last_error()[1]
+    assert lib.mz_call_packed(0, slots, 18) == _native.MZ_ERR_INVALID_ARG
+    assert "takes 19 arguments" in _native.last_error()[1]
+    assert lib.mz_call_packed(0, None, 19) == _native.MZ_ERR_INVALID_ARG
+    wide = [0] * 19
+    wide[7] = 1 << 32  # n_seqs is 32 bits wide
+    with pytest.raises(ValueError, match="out of its type's range"):
+        _native.call_packed("mz_paged_plan", *wide)
+
+
+@pytest.mark.parametrize("name", sorted(_native._PACKED))
+def test_packed_calls_take_their_arguments_in_order(name):
+    """Every argument arrives: each changed one by one from a set that is
+    refused for its sizes gives the status of the plain call."""
+    lib, types = _native.lib(), _native._SIGNATURES[name]
+    assert _native._PACKED[name][2] == len(types)
+    for i in range(-1, len(types)):
+        args = [0.0 if t is ctypes.c_float else 0 for t in types]
+        if i >= 0 and types[i] not in (ctypes.c_void_p, ctypes.c_size_t) and \
+                not issubclass(types[i], ctypes._Pointer):
+            args[i] = -3
+        # pointers stay null and sizes 0 or below: nothing can be launched
+        plain = getattr(lib, name)(*[None if a == 0 and issubclass(
+            t, (ctypes.c_void_p, ctypes._Pointer)) else max(a, 0) if t is ctypes.c_uint32 else a
+            for a, t in zip(args, types)])
+        said = _native.last_error()
+        args = [max(a, 0) if t is ctypes.c_uint32 else a for a, t in zip(args, types)]
+        op, pack, n = _native._PACKED[name]
+        assert lib.mz_call_packed(op, pack(*args), n) == plain != 0
+        assert _native.last_error() == said
