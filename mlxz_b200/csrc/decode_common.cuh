@@ -26,6 +26,7 @@
 #include <cmath>
 #include <cstdlib>
 #include <mutex>
+#include <type_traits>
 
 #include "common.cuh"
 #include "score_mod.cuh"
@@ -416,6 +417,14 @@ struct Sched {
       t_s = tot;
       dyn = 0;
     }
+    if constexpr (std::is_same<P, ModParams>::value) {
+      // A share costs its warp about 1.3 us a tile, a piece its pair's merging warp
+      // 0.1 to 0.4 us: shares below sqrt(n / 5) of n tiles lose more in the merge than
+      // they save (one sequence of 2000 tokens 75 -> 24 us, of 16384 83 -> 61 us); t_s
+      // is tot here, and the last warps get none.
+      if (dyn == 0)
+        per_s = max(per_s, max(2, static_cast<int>(sqrtf(0.2f * static_cast<float>(longest)))));
+    }
     n_chunks = (dyn + chunk - 1) / chunk;
     return true;
   }
@@ -438,6 +447,8 @@ struct Sched {
       }
     }
     while (!ok) {
+      // a split that is all static has no tickets to take
+      if (std::is_same<P, ModParams>::value && n_chunks == 0) return false;
       int tk = 0;
       if (lane == 0) tk = atomicAdd(ticket, 1);
       tk = __shfl_sync(0xffffffffu, tk, 0);
@@ -761,10 +772,104 @@ __device__ __forceinline__ void arrive_or_defer(const Params &p, const Cursor &c
   }
 }
 
+// Merge of many pieces: each row's maximum and the pieces' weights first, so that
+// what a piece costs then is a copy and a multiply-add per element, with the next
+// pieces' copies in flight.  Up to MR rows.  False: `buf` is too small for it.
+// One sequence of 16384 tokens (73 pieces a pair) 61 -> 40 us, of 2000 24 -> 19;
+// few pieces, which one round trip of the staged merge takes, are left to it.
+constexpr int kWeighted = 6;  // pieces from which on it runs
+
+template <int D, int MR>
+__device__ __forceinline__ bool merge_weighted(const Params &p, int b, int h, int uf, int nparts,
+                                               uint8_t *buf, int buf_bytes, int lane) {
+  constexpr int kIt = MR * D / 128;  // 4-element steps per lane
+  const int bh = b * p.Hkv + h, rows = p.rows, E = rows * D;
+  const int part_bytes = E * 4, n = nparts * rows, w_bytes = (8 * n + 15) & ~15;
+  const int per = (buf_bytes - w_bytes) / 2 / part_bytes;  // pieces per stage
+  if (per < 1) return false;
+  const int64_t slot = (int64_t)uf + bh;
+  const uint8_t *src = reinterpret_cast<const uint8_t *>(p.part + slot * E);
+  float2 *mlw = reinterpret_cast<float2 *>(buf);
+  const uint32_t w_s = smem_u32(buf), stage = w_s + w_bytes;
+  auto load = [&](int k0, int s) {
+    const int bytes = min(per, nparts - k0) * part_bytes;  // <= 0: an empty group
+    for (int x = 16 * lane; x < bytes; x += 512)
+      cp_async16(stage + s * per * part_bytes + x, src + (int64_t)k0 * part_bytes + x);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  __syncwarp();  // an earlier merge's reads of buf are done
+  for (int x = lane; x < n; x += 32) cp_async8(w_s + 8 * x, p.ml + (slot * rows + x) * 2);
+  load(0, 0);  // one group with the (m, l)
+  load(per, 1);
+  asm volatile("cp.async.wait_group 1;" ::: "memory");
+  __syncwarp();
+  float inv[kIt];
+#pragma unroll
+  for (int it = 0; it < kIt; ++it) inv[it] = 0.f;
+  for (int r = 0; r < rows; ++r) {
+    float M = -INFINITY, L = 0.f;
+    for (int k = lane; k < nparts; k += 32) M = fmaxf(M, mlw[k * rows + r].x);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    for (int k = lane; k < nparts; k += 32) {
+      const float2 x = mlw[k * rows + r];
+      const float w = fast_exp2(x.x - M);
+      L = fmaf(w, x.y, L);
+      mlw[k * rows + r].x = w;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    const float i = row_inverse(L);
+#pragma unroll
+    for (int it = 0; it < kIt; ++it)
+      if ((4 * lane + 128 * it) / D == r) inv[it] = i;
+  }
+  __syncwarp();
+  float4 acc[kIt];
+#pragma unroll
+  for (int it = 0; it < kIt; ++it) acc[it] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k0 = 0, s = 0; k0 < nparts; k0 += per, s ^= 1) {
+    const float *part = reinterpret_cast<const float *>(buf + w_bytes + s * per * part_bytes);
+    const int cnt = min(per, nparts - k0);
+    for (int k = 0; k < cnt; ++k) {
+#pragma unroll
+      for (int it = 0; it < kIt; ++it) {
+        const int e = 4 * lane + 128 * it;
+        if (e < E) {
+          const float w = mlw[(k0 + k) * rows + e / D].x;
+          const float4 o = *reinterpret_cast<const float4 *>(part + k * E + e);
+          acc[it].x = fmaf(w, o.x, acc[it].x);
+          acc[it].y = fmaf(w, o.y, acc[it].y);
+          acc[it].z = fmaf(w, o.z, acc[it].z);
+          acc[it].w = fmaf(w, o.w, acc[it].w);
+        }
+      }
+    }
+    __syncwarp();
+    load(k0 + 2 * per, s);
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    __syncwarp();
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+  for (int it = 0; it < kIt; ++it) {
+    const int e = 4 * lane + 128 * it;
+    if (e < E) {
+      const int r = e / D, d = e - r * D;
+      const int64_t o = row_offset(p.o_sb, p.o_st, p.o_sh, b, h, r, p.G) + d;
+      store_pair(p, o, acc[it].x * inv[it], acc[it].y * inv[it]);
+      store_pair(p, o + 2, acc[it].z * inv[it], acc[it].w * inv[it]);
+    }
+  }
+  if (lane == 0) p.counters[bh] = 0;
+  return true;
+}
+
 // After the tile loop: run the deferred merges with the idle stage ring `buf`.
 // `ring_idle` false (a wait gave up with copies maybe still landing): leave
-// the outputs and only reset the pairs' counters.
-template <int D, bool GATHER = false>
+// the outputs and only reset the pairs' counters.  MR: rows of the weighted merge
+// (0: the staged one).
+template <int D, bool GATHER = false, int MR = 0>
 __device__ __forceinline__ void run_deferred(const Params &p, const Deferred *dq, int nd,
                                              uint8_t *buf, int buf_bytes, bool ring_idle,
                                              int lane) {
@@ -772,6 +877,9 @@ __device__ __forceinline__ void run_deferred(const Params &p, const Deferred *dq
   for (int j = 0; j < nd; ++j) {
     const Deferred d = dq[j];
     if (ring_idle) {
+      if constexpr (MR > 0)
+        if (d.nparts >= kWeighted &&
+            merge_weighted<D, MR>(p, d.b, d.h, d.uf, d.nparts, buf, buf_bytes, lane)) continue;
       merge_staged<D, GATHER>(p, d.b, d.h, d.uf, d.nparts, buf, buf_bytes, lane);
     } else if (lane == 0) {
       p.counters[d.b * p.Hkv + d.h] = 0;

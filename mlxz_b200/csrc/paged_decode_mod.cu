@@ -417,7 +417,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     advance(ur.cc, p);
     sch.template refill<S>(p, i + 1, issue);
   }
-  run_deferred<D>(p, dq, nd, stages, S * C::kStageBytes, ring_idle, lane);
+  // (with 16 rows the weighted merge's registers cost the loop above 3 %)
+  run_deferred<D, false, RG == 1 ? 8 : 0>(p, dq, nd, stages, S * C::kStageBytes, ring_idle, lane);
 }
 
 template <int D, bool BF16, int RG>

@@ -207,6 +207,30 @@ def test_append_decode_vs_oracle(cuda, batch_invariant, mod):
 
 
 @gpu
+@pytest.mark.parametrize("dtype,D,G,ctx,mod", [
+    ("bf16", 128, 4, [5000], "cap"), ("f16", 64, 8, [9001], "slopes"),
+    ("bf16", 64, 1, [6000, 3], "docs"), ("f16", 128, 2, [3333, 0, 70], "far_sink"),
+    ("bf16", 128, 16, [4100], "prefix"), ("bf16", 128, 8, [16000], "cap")])
+def test_decode_of_few_long_sequences(cuda, dtype, D, G, ctx, mod):
+    """Pairs cut into many pieces: their merge, and warps left without a share."""
+    B, Hkv = len(ctx), 2
+    case = random_paged_case(25, B, Hkv, D, 16, ctx, dtype, G=G)
+    kp, vp, tables, c = _dev(case, dtype, cuda)
+    q = to_dev(case["q"][:, 0], dtype, cuda)
+    kw, ow = _mod_args(MODS[mod], Hkv * G, ctx, np.ones(B, dtype=int), False, cuda)
+    want = osm.paged(case["q"][:, 0], case["kp"], case["vp"], case["tables"], np.arange(B),
+                     np.ones(B, dtype=int), case["ctx"], dtype, **ow)
+    first = None
+    for _ in range(3):
+        out = ops.paged_decode(q, kp, vp, tables, c, out_dtype=torch.float32, **kw)
+        torch.cuda.synchronize()
+        ops.check_device_errors(0)
+        _check(out, want, mod)
+        assert first is None or torch.equal(out, first)
+        first = out
+
+
+@gpu
 def test_batch_invariant_bytes_with_a_window(cuda):
     """A sequence's bytes do not depend on the batch around it."""
     dtype, D, G, Hkv, ctx = "bf16", 64, 4, 2, [3000, 40, 900]
