@@ -630,15 +630,18 @@ __device__ __forceinline__ bool arrive(const Params &p, int bh, int nparts, int 
 }
 
 // Combine of one piece (m, l, O-slice) into the running (M, Ls, acc): the
-// online-softmax merge, pieces taken in slot order.
+// online-softmax merge, pieces taken in slot order.  Which product is rounded
+// ahead of the sum is spelled out: left to the compiler it differed between the
+// staged merge and the one from global memory, and a batch-invariant pair meets
+// the one or the other as its warp's list fills.
 __device__ __forceinline__ void merge_piece(float &M, float &Ls, float4 &acc, float2 ml, float4 o) {
   const float Mn = fmaxf(M, ml.x);
   const float sa = fast_exp2(M - Mn), sb = fast_exp2(ml.x - Mn);
-  Ls = Ls * sa + ml.y * sb;
-  acc.x = acc.x * sa + o.x * sb;
-  acc.y = acc.y * sa + o.y * sb;
-  acc.z = acc.z * sa + o.z * sb;
-  acc.w = acc.w * sa + o.w * sb;
+  Ls = fmaf(ml.y, sb, __fmul_rn(Ls, sa));
+  acc.x = fmaf(o.x, sb, __fmul_rn(acc.x, sa));
+  acc.y = fmaf(o.y, sb, __fmul_rn(acc.y, sa));
+  acc.z = fmaf(o.z, sb, __fmul_rn(acc.z, sa));
+  acc.w = fmaf(o.w, sb, __fmul_rn(acc.w, sa));
   M = Mn;
 }
 

@@ -761,3 +761,35 @@ def test_negative_slopes_raise_far_scores(cuda, softcap):
     last = case["q_start"] + case["q_len"] - 1
     out = ops.paged_decode(to_dev(case["qp"][last], dtype, cuda), kp, vp, tables, c, **kw)
     _check(out, (want[0][last], want[1][last]))
+
+
+def _torch_pools(cuda, seed, n_blocks, Hkv, bs, D, dtype=torch.bfloat16):
+    g = torch.Generator(device=cuda).manual_seed(seed)
+    return (torch.randn(n_blocks, Hkv, bs, D, generator=g, device=cuda).to(dtype) for _ in range(2))
+
+
+@gpu
+@pytest.mark.parametrize("D,G,kw", [(128, 1, dict(softcap=30.0)), (64, 16, dict(softcap=30.0)),
+                                    (128, 4, {}), (64, 8, {}), (128, 16, {}), (64, 16, {})])
+def test_batch_invariant_bytes_with_many_merges_a_warp(cuda, D, G, kw):
+    """A sequence's bytes do not depend on the batch around it, nor on the run,
+    where its pieces are many (3500 tokens: seven) and a warp merges more pairs
+    than its list of eight holds (24 sequences of 4 KV heads on 8 warps)."""
+    B, Hkv, bs = 24, 4, 16
+    ctx = [3500 - 7 * b for b in range(B)]
+    width = -(-max(ctx) // bs)
+    kp, vp = _torch_pools(cuda, 71, B * width, Hkv, bs, D)
+    tables = torch.randperm(B * width, generator=torch.Generator().manual_seed(72)).int()
+    tables = tables.reshape(B, width).to(cuda)
+    c = torch.tensor(ctx, dtype=torch.int32, device=cuda)
+    g = torch.Generator(device=cuda).manual_seed(73)
+    q = torch.randn(B, Hkv * G, D, generator=g, device=cuda).to(kp.dtype)
+    kn, vn = (torch.randn(B, Hkv, D, generator=g, device=cuda).to(kp.dtype) for _ in range(2))
+    kw = dict(kw, batch_invariant=True, num_warps=8, out_dtype=torch.float32)
+    runs = [ops.paged_append_decode(q, kp, vp, kn, vn, tables, c, **kw) for _ in range(4)]
+    for b in range(0, B, 3):
+        s = slice(b, b + 1)
+        one = ops.paged_append_decode(q[s], kp, vp, kn[s], vn[s], tables[s].contiguous(), c[s], **kw)
+        for out in runs:
+            assert torch.equal(one[0], out[b]), b
+    ops.check_device_errors(0)
