@@ -609,7 +609,8 @@ struct UnitReader {
 // streaming; when its tile loop is over (its stage ring idle) it runs the list,
 // staging each pair's partials into the ring with cp.async -- one round trip
 // for all of them -- and combining them from shared memory.  A list that is
-// full falls back to merging at once from global memory.
+// full falls back to merging at once from global memory, with the same sums in
+// the same order: a pair's bytes do not depend on who merges it.
 // ---------------------------------------------------------------------------
 constexpr int kMaxDeferred = 8;  // deferred merges per warp
 
@@ -758,38 +759,40 @@ __device__ __forceinline__ void merge_staged(const Params &p, int b, int h, int 
   if (lane == 0) p.counters[bh] = 0;
 }
 
-// In the tile loop, after this warp's piece of the pair has been written.
-// Small merges (rows * pieces <= kMergeNow) run at once; larger ones are
-// deferred while the list has room.
-constexpr int kMergeNow = 16;
-
-template <int D, bool GATHER = false>
-__device__ __forceinline__ void arrive_or_defer(const Params &p, const Cursor &cc, int bh, int uf,
-                                                int nparts, int lane, Deferred *dq, int &nd) {
-  if (!arrive(p, bh, nparts, lane)) return;
-  if (p.rows * nparts > kMergeNow && nd < kMaxDeferred) {
-    if (lane == 0) dq[nd] = Deferred{cc.b, cc.h, uf, nparts};
-    ++nd;
-  } else {
-    merge_global<D, GATHER>(p, cc.b, cc.h, uf, nparts, lane);
-  }
-}
+constexpr int kMergeNow = 16;  // rows * pieces up to which a merge runs at once
 
 // Merge of many pieces: each row's maximum and the pieces' weights first, so that
 // what a piece costs then is a copy and a multiply-add per element, with the next
-// pieces' copies in flight.  Up to MR rows.  False: `buf` is too small for it.
+// pieces' copies in flight.  Up to MR rows.
 // One sequence of 16384 tokens (73 pieces a pair) 61 -> 40 us, of 2000 24 -> 19;
 // few pieces, which one round trip of the staged merge takes, are left to it.
 constexpr int kWeighted = 6;  // pieces from which on it runs
 
+// Bytes of the (m, l) of a pair's pieces in the weighted merge's buffer, and the
+// pieces that a stage behind them takes.
+__device__ __forceinline__ int weight_bytes(const Params &p, int nparts) {
+  return (8 * nparts * p.rows + 15) & ~15;
+}
+template <int D>
+__device__ __forceinline__ int weighted_per(const Params &p, int nparts, int buf_bytes) {
+  return (buf_bytes - weight_bytes(p, nparts)) / 2 / (p.rows * D * 4);
+}
+
+// Whether a pair's merge is the weighted one: by the pair alone, so that its bytes
+// do not depend on which warp merges it, or when.
+template <int D>
+__device__ __forceinline__ bool takes_weights(const Params &p, int nparts, int buf_bytes) {
+  return p.rows * nparts > kMergeNow && nparts >= kWeighted &&
+         weighted_per<D>(p, nparts, buf_bytes) >= 1;
+}
+
 template <int D, int MR>
-__device__ __forceinline__ bool merge_weighted(const Params &p, int b, int h, int uf, int nparts,
+__device__ __forceinline__ void merge_weighted(const Params &p, int b, int h, int uf, int nparts,
                                                uint8_t *buf, int buf_bytes, int lane) {
   constexpr int kIt = MR * D / 128;  // 4-element steps per lane
   const int bh = b * p.Hkv + h, rows = p.rows, E = rows * D;
-  const int part_bytes = E * 4, n = nparts * rows, w_bytes = (8 * n + 15) & ~15;
-  const int per = (buf_bytes - w_bytes) / 2 / part_bytes;  // pieces per stage
-  if (per < 1) return false;
+  const int part_bytes = E * 4, n = nparts * rows, w_bytes = weight_bytes(p, nparts);
+  const int per = weighted_per<D>(p, nparts, buf_bytes);  // pieces per stage
   const int64_t slot = (int64_t)uf + bh;
   const uint8_t *src = reinterpret_cast<const uint8_t *>(p.part + slot * E);
   float2 *mlw = reinterpret_cast<float2 *>(buf);
@@ -865,7 +868,69 @@ __device__ __forceinline__ bool merge_weighted(const Params &p, int b, int h, in
     }
   }
   if (lane == 0) p.counters[bh] = 0;
-  return true;
+}
+
+// The same sums in the same order straight from global memory, a row at a time:
+// for a warp whose list is full while its ring is still in use.
+template <int D>
+__device__ __forceinline__ void merge_weighted_global(const Params &p, int b, int h, int uf,
+                                                      int nparts, int lane) {
+  const int bh = b * p.Hkv + h;
+  const int64_t slot = (int64_t)uf + bh;
+  for (int r = 0; r < p.rows; ++r) {
+    const float *ml = p.ml + (slot * p.rows + r) * 2;  // piece k's: 2 k rows further
+    const float *part = p.part + (slot * p.rows + r) * D;
+    float M = -INFINITY, L = 0.f;
+    for (int k = lane; k < nparts; k += 32) M = fmaxf(M, __ldcg(ml + 2 * k * p.rows));
+#pragma unroll
+    for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    for (int k = lane; k < nparts; k += 32) {
+      const float2 x = __ldcg(reinterpret_cast<const float2 *>(ml + 2 * k * p.rows));
+      L = fmaf(fast_exp2(x.x - M), x.y, L);
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    const float inv = row_inverse(L);
+    const int d = 4 * lane;
+    if (d < D) {
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = 0; k < nparts; ++k) {
+        const float w = fast_exp2(__ldcg(ml + 2 * k * p.rows) - M);
+        const float4 x = __ldcg(reinterpret_cast<const float4 *>(part + (int64_t)k * p.rows * D + d));
+        acc.x = fmaf(w, x.x, acc.x);
+        acc.y = fmaf(w, x.y, acc.y);
+        acc.z = fmaf(w, x.z, acc.z);
+        acc.w = fmaf(w, x.w, acc.w);
+      }
+      const int64_t o = row_offset(p.o_sb, p.o_st, p.o_sh, b, h, r, p.G) + d;
+      store_pair(p, o, acc.x * inv, acc.y * inv);
+      store_pair(p, o + 2, acc.z * inv, acc.w * inv);
+    }
+  }
+  if (lane == 0) p.counters[bh] = 0;
+}
+
+
+// In the tile loop, after this warp's piece of the pair has been written.
+// Small merges (rows * pieces <= kMergeNow) run at once; larger ones are
+// deferred while the list has room.  MR, buf_bytes: as in run_deferred.
+template <int D, bool GATHER = false, int MR = 0>
+__device__ __forceinline__ void arrive_or_defer(const Params &p, const Cursor &cc, int bh, int uf,
+                                                int nparts, int lane, Deferred *dq, int &nd,
+                                                int buf_bytes = 0) {
+  if (!arrive(p, bh, nparts, lane)) return;
+  if (p.rows * nparts > kMergeNow && nd < kMaxDeferred) {
+    if (lane == 0) dq[nd] = Deferred{cc.b, cc.h, uf, nparts};
+    ++nd;
+  } else {
+    if constexpr (MR > 0) {
+      if (takes_weights<D>(p, nparts, buf_bytes)) {
+        merge_weighted_global<D>(p, cc.b, cc.h, uf, nparts, lane);
+        return;
+      }
+    }
+    merge_global<D, GATHER>(p, cc.b, cc.h, uf, nparts, lane);
+  }
 }
 
 // After the tile loop: run the deferred merges with the idle stage ring `buf`.
@@ -880,9 +945,12 @@ __device__ __forceinline__ void run_deferred(const Params &p, const Deferred *dq
   for (int j = 0; j < nd; ++j) {
     const Deferred d = dq[j];
     if (ring_idle) {
-      if constexpr (MR > 0)
-        if (d.nparts >= kWeighted &&
-            merge_weighted<D, MR>(p, d.b, d.h, d.uf, d.nparts, buf, buf_bytes, lane)) continue;
+      if constexpr (MR > 0) {
+        if (takes_weights<D>(p, d.nparts, buf_bytes)) {
+          merge_weighted<D, MR>(p, d.b, d.h, d.uf, d.nparts, buf, buf_bytes, lane);
+          continue;
+        }
+      }
       merge_staged<D, GATHER>(p, d.b, d.h, d.uf, d.nparts, buf, buf_bytes, lane);
     } else if (lane == 0) {
       p.counters[d.b * p.Hkv + d.h] = 0;

@@ -73,6 +73,8 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
   using C = ModCfg<D>;
   constexpr int S = C::kStages;
   constexpr int KS = D / 16;  // k-steps of K.Q^T, m-tiles of V^T.P^T
+  // rows of the weighted merge (with 16 its registers cost the tile loop 3 %)
+  constexpr int kMergeRows = RG == 1 ? 8 : 0;
 
   launch_dependents();
   extern __shared__ uint8_t smem_raw[];
@@ -408,7 +410,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
             }
           }
         }
-      if (!whole) arrive_or_defer<D>(p, cc, bh, uf, ul - uf + 1, lane, dq, nd);
+      if (!whole)
+        arrive_or_defer<D, false, kMergeRows>(p, cc, bh, uf, ul - uf + 1, lane, dq, nd,
+                                              S * C::kStageBytes);
       seg_first = true;  // the next tile starts a new piece
     }
 
@@ -417,8 +421,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     advance(ur.cc, p);
     sch.template refill<S>(p, i + 1, issue);
   }
-  // (with 16 rows the weighted merge's registers cost the loop above 3 %)
-  run_deferred<D, false, RG == 1 ? 8 : 0>(p, dq, nd, stages, S * C::kStageBytes, ring_idle, lane);
+  run_deferred<D, false, kMergeRows>(p, dq, nd, stages, S * C::kStageBytes, ring_idle, lane);
 }
 
 template <int D, bool BF16, int RG>

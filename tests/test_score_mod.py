@@ -769,7 +769,8 @@ def _torch_pools(cuda, seed, n_blocks, Hkv, bs, D, dtype=torch.bfloat16):
 
 
 @gpu
-@pytest.mark.parametrize("D,G,kw", [(128, 1, dict(softcap=30.0)), (64, 16, dict(softcap=30.0)),
+@pytest.mark.parametrize("D,G,kw", [(128, 4, dict(softcap=30.0)), (64, 8, dict(window=3400)),
+                                    (128, 1, dict(softcap=30.0)), (64, 16, dict(softcap=30.0)),
                                     (128, 4, {}), (64, 8, {}), (128, 16, {}), (64, 16, {})])
 def test_batch_invariant_bytes_with_many_merges_a_warp(cuda, D, G, kw):
     """A sequence's bytes do not depend on the batch around it, nor on the run,
