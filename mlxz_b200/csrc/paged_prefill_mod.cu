@@ -134,7 +134,8 @@ __device__ __forceinline__ bool item_at(const PParams &p, Walk &w, int e, Item &
     }
     const int b = w.b + lane;
     n = b < p.n_seqs ? max(0, p.q_len[b]) : 0;
-    blocks = min((n + tpc - 1) / tpc, p.qblocks);
+    // (a length near 2^31 must not overflow: its sequence is reported below)
+    blocks = min(n / tpc + (n % tpc != 0), p.qblocks);
     const int mine = blocks * p.Hkv;
     int incl = mine;
 #pragma unroll

@@ -794,3 +794,26 @@ def test_batch_invariant_bytes_with_many_merges_a_warp(cuda, D, G, kw):
         for out in runs:
             assert torch.equal(one[0], out[b]), b
     ops.check_device_errors(0)
+
+
+@gpu
+@pytest.mark.parametrize("ctx", [[300, 130, 4300], [4300, 1, 4300]])
+@pytest.mark.parametrize("n", [(1 << 31) - 1, (1 << 31) - 16, 1 << 30, 301])
+def test_prefill_reports_a_length_of_any_size(cuda, ctx, n):
+    """A sequence whose query length on the device exceeds its context, up to
+    2^31 - 1, is reported; the sequences behind it are computed all the same."""
+    qlen = [20, 1, 33]
+    case = _prefill_case(64, ctx, qlen, "bf16", 64, 4, 16, 2)
+    kp, vp, tables, c = _dev(case, "bf16", cuda)
+    c[0] = 300
+    lens = torch.tensor([n, 1, 33], dtype=torch.int32, device=cuda)
+    starts = torch.from_numpy(case["q_start"]).to(cuda)
+    out = torch.full((54, 8, 64), 7.0, dtype=torch.bfloat16, device=cuda)
+    ops.paged_prefill(to_dev(case["qp"], "bf16", cuda), kp, vp, tables, starts, lens, c, 33,
+                      softcap=20.0, out=out)
+    with pytest.raises(DeviceError, match="context length"):
+        ops.check_device_errors(0)
+    assert (out[:20] == 7).all()
+    want = osm.paged(case["qp"], case["kp"], case["vp"], case["tables"], case["q_start"],
+                     case["q_len"], case["ctx"], "bf16", softcap=20.0)
+    _check(out[20:], (want[0][20:], want[1][20:]))
