@@ -817,3 +817,30 @@ def test_prefill_reports_a_length_of_any_size(cuda, ctx, n):
     want = osm.paged(case["qp"], case["kp"], case["vp"], case["tables"], case["q_start"],
                      case["q_len"], case["ctx"], "bf16", softcap=20.0)
     _check(out[20:], (want[0][20:], want[1][20:]))
+
+
+@gpu
+@pytest.mark.parametrize("window", [1, 100, 4000])
+@pytest.mark.parametrize("ctx", [(1 << 31) - 2048, (1 << 31) - 2048 - 1000])
+def test_window_over_the_longest_context(cuda, window, ctx):
+    """The widest table that is taken (2^31 - 2048 tokens): the block ids that are
+    loaded ahead end behind the last key, and past 2^31.  All its entries are
+    one block of 1024 tokens, so a short cache of the same block has the same
+    keys in the window."""
+    D, bs, G, n = 64, 1024, 2, 3
+    case = random_paged_case(65, 1, 1, D, bs, [bs], "bf16", n_blocks=1, G=G)
+    kp, vp = (to_dev(case[k], "bf16", cuda) for k in ("kp", "vp"))
+    case["qp"] = rng.normal(65, (n, G, D), "bf16", stream=9)
+    q = to_dev(case["qp"], "bf16", cuda)
+    tables = torch.zeros(1, (1 << 21) - 2, dtype=torch.int32, device=cuda)
+    short = 8192 - ((1 << 31) - ctx) % bs
+    want = osm.paged(case["qp"], case["kp"], case["vp"], np.zeros((1, 8), dtype=np.int32),
+                     np.array([0]), np.array([n]), np.array([short]), "bf16", window=window)
+    c = torch.tensor([ctx], dtype=torch.int32, device=cuda)
+    i = [torch.tensor([x], dtype=torch.int32, device=cuda) for x in (0, n)]
+    out = ops.paged_prefill(q, kp, vp, tables, *i, c, n, window=window)
+    ops.check_device_errors(0)
+    _check(out, want)
+    out = ops.paged_decode(q[None], kp, vp, tables, c, window=window, causal=True)
+    ops.check_device_errors(0)
+    _check(out[0], want)
