@@ -1064,7 +1064,6 @@ extern "C" int mz_paged_prefill(void *out, int32_t out_dtype, int64_t out_tok_st
   if (empty) return MZ_OK;
 
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const int tpc = kM / (n_heads / n_kv_heads);
   const bool bf16 = dtype == MZ_DTYPE_BF16;
   // The persistent form (one CTA per SM over all query blocks) by default;
   // MLXZ_B200_PREFILL_PERSIST=0 launches one CTA per query block instead
@@ -1089,7 +1088,7 @@ extern "C" int mz_paged_prefill(void *out, int32_t out_dtype, int64_t out_tok_st
     MZ_CHECK_LAUNCH(fn);
     return MZ_OK;
   }
-  const dim3 grid((max_q_len + tpc - 1) / tpc, n_kv_heads, n_seqs);
+  const dim3 grid(p.qblocks, n_kv_heads, n_seqs);
 #define MZ_TCLAUNCH(D_, BF_)                                                                     \
   do {                                                                                           \
     if (int rc = smem_attr_tc<D_, BF_>()) return rc;                                             \

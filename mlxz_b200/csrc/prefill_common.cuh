@@ -145,11 +145,11 @@ inline int prepare(PParams *p, CUtensorMap *tk, CUtensorMap *tv, bool *empty, in
   p->scale_log2 = static_cast<float>(static_cast<double>(scale) * 1.4426950408889634);
   p->sub_log2 = sub_log2;
   p->err = dev_err;
-  if (n_seqs > 65535 || n_kv_heads > 65535 || max_q_len > (1 << 30))
+  if (n_seqs > 65535 || n_kv_heads > 65535)
     return fail(MZ_ERR_UNSUPPORTED, "%s: grid too large", fn);
   const int tpc = kM / G;
   p->n_seqs = n_seqs;
-  p->qblocks = (max_q_len + tpc - 1) / tpc;
+  p->qblocks = (max_q_len - 1) / tpc + 1;  // (any bound up to 2^31 - 1 is taken)
   return MZ_OK;
 }
 

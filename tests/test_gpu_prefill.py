@@ -244,3 +244,18 @@ def test_chunked_prefill_step_matches_whole_prompt(cuda):
             ref = opaged.attention(rng.to_f32(qd[l, b][:, None], dtype), rng.to_f32(kk, dtype),
                                    rng.to_f32(vv, dtype))[:, 0]
             assert attn_err(out[l, b], ref) <= ATOL_REL, (s, l)
+
+
+@pytest.mark.parametrize("max_q_len", [(1 << 30) + 1, (1 << 31) - 128, (1 << 31) - 1])
+@pytest.mark.parametrize("kw", [{}, dict(window=40)])
+def test_any_bound_on_the_query_lengths_is_taken(cuda, max_q_len, kw):
+    """max_q_len is a bound: one far above the chunks gives the bytes of a close
+    one (modified scores share keys out by it: the same values)."""
+    dtype, D, ctx, qlen = "bf16", 64, [100], [37]
+    case = _prefill_case(19, ctx, qlen, dtype, D, 1, 16, 1)
+    dev = [torch.from_numpy(case[k]).to(cuda) for k in ("tables", "q_start", "q_len", "ctx")]
+    pools = [to_dev(case[k], dtype, cuda) for k in ("kp", "vp")]
+    q = to_dev(case["qp"], dtype, cuda)
+    want, out = (ops.paged_prefill(q, *pools, *dev, m, **kw) for m in (37, max_q_len))
+    ops.check_device_errors(0)
+    assert torch.equal(out, want) if not kw else attn_err(out, want.float().cpu().numpy()) <= ATOL_REL
