@@ -1069,9 +1069,11 @@ extern "C" int mz_paged_prefill(void *out, int32_t out_dtype, int64_t out_tok_st
   // MLXZ_B200_PREFILL_PERSIST=0 launches one CTA per query block instead
   if (decode::env_int("MLXZ_B200_PREFILL_PERSIST", 1, 0, 1) == 1) {
     const int64_t items = (int64_t)n_seqs * n_kv_heads * p.qblocks;
-    if (items >= (int64_t(1) << 31)) return fail(MZ_ERR_UNSUPPORTED, "%s: too many query blocks", fn);
     const int sms = sm_count(current_device());
     if (sms <= 0) return fail(MZ_ERR_CUDA, "%s: cannot query the SM count", fn);
+    // (a CTA counts its items past the last one)
+    if (items + sms >= (int64_t(1) << 31))
+      return fail(MZ_ERR_UNSUPPORTED, "%s: too many query blocks", fn);
     const dim3 grid_ps(static_cast<unsigned>(std::min<int64_t>(items, sms)));
 #define MZ_PSLAUNCH(D_, BF_)                                                                     \
   do {                                                                                           \

@@ -259,3 +259,16 @@ def test_any_bound_on_the_query_lengths_is_taken(cuda, max_q_len, kw):
     want, out = (ops.paged_prefill(q, *pools, *dev, m, **kw) for m in (37, max_q_len))
     ops.check_device_errors(0)
     assert torch.equal(out, want) if not kw else attn_err(out, want.float().cpu().numpy()) <= ATOL_REL
+
+
+@pytest.mark.parametrize("max_q_len", [1 << 30, (1 << 30) - 5])
+@pytest.mark.parametrize("kw", [{}, dict(window=40)])
+def test_too_many_query_blocks_are_refused(cuda, max_q_len, kw):
+    """Item numbers are ints, also those past the last item that end a CTA's
+    loop: 2^31 items and 2^31 - 10 (two sequences, a token per item)."""
+    dtype, D, G, ctx, qlen = "bf16", 64, 128, [20, 20], [3, 3]
+    case = _prefill_case(20, ctx, qlen, dtype, D, G, 16, 1)
+    dev = [torch.from_numpy(case[k]).to(cuda) for k in ("tables", "q_start", "q_len", "ctx")]
+    pools = [to_dev(case[k], dtype, cuda) for k in ("kp", "vp")]
+    with pytest.raises(NativeError, match="too many query blocks"):
+        ops.paged_prefill(to_dev(case["qp"], dtype, cuda), *pools, *dev, max_q_len, **kw)
