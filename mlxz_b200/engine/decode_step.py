@@ -231,10 +231,11 @@ class PagedDecodeStep:
         self.tables.copy_(host, non_blocking=False)
         self.positions.copy_(offs)
         self.lengths.copy_(offs + 1)
-        # offsets and blocks of each table that the device has
+        # offsets and tables that the device has
         self._offsets = offs.tolist()
-        self._uploaded = [len(self.store.tables[s]) for s in self.seq_ids]
-        self._held = torch.tensor(self._uploaded, dtype=torch.int32).to(self.store.device)
+        self._uploaded = [list(self.store.tables[s]) for s in self.seq_ids]
+        self._held = torch.tensor([len(t) for t in self._uploaded],
+                                  dtype=torch.int32).to(self.store.device)
 
     @property
     def plain(self) -> bool:
@@ -297,7 +298,8 @@ class PagedDecodeStep:
 
     def advance(self) -> None:
         """Commit the appended token: offsets += 1, growing tables as needed.
-        New blocks' ids go up alone; mz_paged_plan puts them into the tables."""
+        New blocks' ids go up alone; mz_paged_plan puts them into the tables.
+        Tables or offsets that also changed by other hands go up whole."""
         st = self.store
         new: list[int] = []
         in_step = True  # the device's tables are what the host's were before
@@ -306,9 +308,10 @@ class PagedDecodeStep:
             had = len(st.tables[s])
             st.ensure_capacity(s, 1)
             new += st.tables[s][had:]
-            in_step &= (had == self._uploaded[i] and st.offsets[s] == self._offsets[i] + 1
+            in_step &= (had == len(self._uploaded[i]) and st.offsets[s] == self._offsets[i] + 1
                         and len(st.tables[s]) <= self.max_blocks)
-        if new and not in_step:
+        if new and not (in_step and all(st.tables[s][:len(up)] == up
+                                        for s, up in zip(self.seq_ids, self._uploaded))):
             self.sync_metadata()
             return
         self._offsets = [o + 1 for o in self._offsets]
@@ -321,7 +324,8 @@ class PagedDecodeStep:
             plan = ops.paged_plan(self.tables, self.positions, self._ones, self.B, st.block_size,
                                   st.n_blocks, new_ids=ids, held=self._held)
             self._held = plan.held
-            self._uploaded = [len(st.tables[s]) for s in self.seq_ids]
+            for s, up in zip(self.seq_ids, self._uploaded):
+                up += st.tables[s][len(up):]
 
     _ones: torch.Tensor | None = None
 

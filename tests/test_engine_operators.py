@@ -201,6 +201,36 @@ def test_advance_with_offsets_from_outside(cuda):
         tb = store.tables[s]
         assert step.tables[i].tolist() == tb + [-1] * (4 - len(tb))
 
+@gpu
+def test_advance_with_blocks_exchanged_from_outside(cuda):
+    """Blocks that were exchanged between steps (a copy on write by another
+    path, a request put in another's place) go up with the next block."""
+    store = PagedKVStore(1, 64, HKV, D, BS, torch.bfloat16, cuda)
+    store.add_sequence("a", 14)
+    store.add_sequence("b", 40)
+    step = PagedDecodeStep(store, ["a", "b"], HQ, max_blocks=4)
+    store.tables["b"][1] = store.bm.allocate(1)[0]
+
+    def same():
+        for i, s in enumerate(("a", "b")):
+            tb = store.tables[s]
+            assert step.tables[i].tolist() == tb + [-1] * (4 - len(tb))
+        assert step.positions.tolist() == [store.offsets[s] for s in ("a", "b")]
+
+    step.advance()
+    step.advance()  # "a" grows
+    assert len(store.tables["a"]) == 2
+    same()
+    store.free_sequence("b")
+    store.bm.allocate(1)
+    store.add_sequence("b", 42)  # as many tokens in as many blocks, but others
+    while store.offsets["b"] < 48:
+        step.advance()  # "b" grows
+    assert len(store.tables["b"]) == 4
+    same()
+    torch.cuda.synchronize()
+    ops.check_device_errors(0)
+
 
 def test_fused_all_gather_takes_plain_steps_only():
     class Step:
