@@ -139,6 +139,8 @@ class PagedPrefillStep:
         if dev.type == "cuda":
             plan = ops.paged_plan(self.tables, cached, self.q_len, self.T, store.block_size,
                                   store.n_blocks, held=held)
+            # like the uploads it is done here: the layers may run on another stream
+            torch.cuda.current_stream(dev).synchronize()
         else:  # a store without a GPU: metadata alone, no layer runs
             plan = self._host_plan(lens)
         self.q_start, self.ctx_lens, self.slots = plan.q_start, plan.lengths, plan.slots

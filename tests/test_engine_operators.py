@@ -231,6 +231,31 @@ def test_advance_with_blocks_exchanged_from_outside(cuda):
     torch.cuda.synchronize()
     ops.check_device_errors(0)
 
+@gpu
+def test_prefill_metadata_is_done_when_the_step_is_made(cuda, monkeypatch):
+    """A step made on one stream may run its layers on another at once: what it
+    holds on the device is complete, like the uploads of its tables."""
+    plan = ops.paged_plan
+
+    def late(*args, **kw):
+        torch.cuda._sleep(200_000_000)  # about 0.1 s ahead of the launch
+        return plan(*args, **kw)
+
+    store = PagedKVStore(1, 8, HKV, D, BS, torch.bfloat16, cuda)
+    store.add_sequence("x")
+    made = torch.cuda.Stream()
+    with torch.cuda.stream(made):
+        PagedPrefillStep(store, [("x", 40)], HQ)  # the kernel's first launch may wait by itself
+        monkeypatch.setattr(ops, "paged_plan", late)
+        step = PagedPrefillStep(store, [("x", 40)], HQ)
+        assert made.query()
+    q, k, v = (to_dev(t[0], DT, cuda) for t in _tokens(40, 3))
+    out = step.layer(0, q, k, v)
+    ops.check_device_errors(0)
+    f = [rng.to_f32(to_bits(x), DT).transpose(1, 0, 2) for x in (q, k, v)]
+    o, sp = osm.attention(*f, np.arange(40), D ** -0.5)
+    _check(out, o.transpose(1, 0, 2), sp.transpose(1, 0, 2))
+
 
 def test_fused_all_gather_takes_plain_steps_only():
     class Step:
