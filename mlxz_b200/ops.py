@@ -22,6 +22,8 @@ _DTYPES = {torch.float16: nat.MZ_DTYPE_F16, torch.bfloat16: nat.MZ_DTYPE_BF16,
            torch.float32: nat.MZ_DTYPE_F32}
 _DEBUG = os.environ.get("MLXZ_B200_DEBUG", "0") not in ("", "0")
 
+_F32_TINY = torch.finfo(torch.float32).tiny
+
 _err_words: dict[int, torch.Tensor] = {}
 # Decode workspaces handed out when the caller passes none, one per exact
 # problem layout.  The kernels need the arrival counters and scheduler words at
@@ -459,6 +461,8 @@ def _score_mod(q: torch.Tensor, n_heads: int, softcap: float,
     is in use (the sink tokens alone change nothing)."""
     if softcap < 0 or not math.isfinite(softcap):
         raise ValueError("softcap must be finite and not negative (0: none)")
+    if 0 < softcap < _F32_TINY:  # as a float32 it could become 0, which is none
+        raise ValueError(f"softcap must be 0 (none) or at least {_F32_TINY}")
     if window < 0 or sink_tokens < 0:
         raise ValueError("window and sink_tokens must not be negative")
     if not (softcap or window) and alibi_slopes is None and prefix_lens is None and \
@@ -474,7 +478,7 @@ def _score_mod(q: torch.Tensor, n_heads: int, softcap: float,
             _as_i32(t, q.device, name)
             raise ValueError(f"{name} must hold {n} entries")
     big = (1 << 31) - 1
-    return nat.ScoreMod(softcap, min(window, big), min(sink_tokens, big), _ptr(alibi_slopes),
+    return nat.ScoreMod(min(softcap, 1e38), min(window, big), min(sink_tokens, big), _ptr(alibi_slopes),
                         _ptr(prefix_lens), _ptr(first_keys))
 
 

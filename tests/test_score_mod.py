@@ -844,3 +844,26 @@ def test_window_over_the_longest_context(cuda, window, ctx):
     out = ops.paged_decode(q[None], kp, vp, tables, c, window=window, causal=True)
     ops.check_device_errors(0)
     _check(out[0], want)
+
+
+@pytest.mark.parametrize("softcap", [1e-50, 1e-40, 5e-324])
+def test_caps_below_float32_are_refused(softcap):
+    """Rounded to float32 they would be 0, which stands for no cap."""
+    q, kp, vp, tables, ctx = _host()
+    with pytest.raises(ValueError, match="softcap"):
+        ops.paged_decode(q, kp, vp, tables, ctx, softcap=softcap)
+    with pytest.raises(ValueError, match="softcap"):
+        ops.paged_prefill(q, kp, vp, tables, ctx, ctx, ctx, 1, softcap=softcap)
+
+
+@gpu
+def test_caps_beyond_float32_are_none(cuda):
+    q, kp, vp, tables, ctx = (t.to(cuda) for t in _host())
+    q, kp, ctx = torch.randn_like(q), torch.randn_like(kp), ctx + 20
+    tables[:] = torch.arange(4, device=cuda).reshape(2, 2)
+    vp = torch.randn_like(vp)
+    slopes = torch.zeros(8, device=cuda)
+    a, b = (ops.paged_decode(q, kp, vp, tables, ctx, softcap=c, alibi_slopes=slopes)
+            for c in (1e300, 0.0))
+    ops.check_device_errors(0)
+    assert torch.equal(a, b)
