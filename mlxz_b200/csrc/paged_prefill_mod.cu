@@ -135,7 +135,7 @@ __device__ __forceinline__ bool item_at(const PParams &p, Walk &w, int e, Item &
     const int b = w.b + lane;
     n = b < p.n_seqs ? max(0, p.q_len[b]) : 0;
     // (a length near 2^31 must not overflow: its sequence is reported below)
-    blocks = min(n / tpc + (n % tpc != 0), p.qblocks);
+    blocks = min((min(n, INT_MAX - kM) + tpc - 1) / tpc, p.qblocks);
     const int mine = blocks * p.Hkv;
     int incl = mine;
 #pragma unroll
@@ -383,21 +383,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     int k_issued = 0, v_issued = 0;
     for (; ok && have; e += e_step, have = next_item(e, it)) {
       // lane l holds box l % nst of tile per * x + l / nst; block ids are loaded
-      // one such set ahead of their use.  A set ends up to 4095 keys behind the last
-      // one, which with contexts near 2^31 is past the largest int: -1 stands for
-      // keys behind the last one.
-      auto box_key = [&](int x) -> int {
-        const unsigned t = static_cast<unsigned>(it.template own<SPLIT>(per * x + (lane >> nst_log2))) * kN +
-                           (lane & (nst - 1)) * sub;
-        return t < static_cast<unsigned>(it.kv_len) ? static_cast<int>(t) : -1;
+      // one such set ahead of their use.  Sets end behind the last tile: the tile
+      // next to it stands for all of those, whose keys could pass 2^31.
+      auto box_key = [&](int x) {
+        const int t = min(per * x + (lane >> nst_log2), it.ntiles);
+        return it.template own<SPLIT>(t) * kN + (lane & (nst - 1)) * sub;
       };
       auto ids = [&](int x) -> int32_t {
         const int t = box_key(x);
-        return t >= 0 ? p.tables[(int64_t)it.b * p.max_blocks + t / p.bs] : 0;
+        return t < it.kv_len ? p.tables[(int64_t)it.b * p.max_blocks + t / p.bs] : 0;
       };
       auto rows = [&](int x, int32_t blk) -> int {
         const int t = box_key(x);
-        if (t < 0) return 0;
+        if (t >= it.kv_len) return 0;
         if (blk < 0 || blk >= p.n_blocks) {
           // a box that no row sees may have lost its block: any block will do
           if (t < it.head || t + sub > it.lo) dev_error(p.err, MZ_DEVERR_BLOCK_ID);
