@@ -291,10 +291,13 @@ MZ_API int mz_paged_prefill(void *out, int32_t out_dtype, int64_t out_tok_stride
  * window 0 for no window, and first = first_keys[sequence] in the decode calls,
  * first_keys[row of q] in mz_paged_prefill_mod (NULL: 0; the document mask: the
  * position at which the token's document starts).  A token that sees no key
- * gets zeros.  Blocks that no token of the call sees are not read: their
- * table entries may be stale.  All arrays are on the device; like ctx_lens,
- * the kernel ahead of a launch with MZ_LAUNCH_OVERLAP_PREVIOUS must not write
- * them.  The cap is off by at most 2.4e-7 * softcap, above a cap of 1000 by 1e-6
+ * gets zeros.  Blocks behind the prefix and the sinks and below the lowest
+ * max(first, p - window + 1) of the sequence's tokens in the call are not read:
+ * their table entries may be stale, their keys and values anything.  Sink
+ * tokens are the sequence's first ones: packed documents all see them.  All
+ * arrays are on the device; like ctx_lens, the kernel ahead of a launch with
+ * MZ_LAUNCH_OVERLAP_PREVIOUS must not write them.  Distances and their bias are
+ * fp32.  The cap is off by at most 2.4e-7 * softcap, above a cap of 1000 by 1e-6
  * of the score; a cap from 1e30 on is none.  Same
  * place in the reference as the unmodified calls: the scaled dot product
  * attention of src/mlxz/paged_attention/attention.py:40-42, whose models mask
@@ -356,14 +359,14 @@ MZ_API int mz_paged_prefill_mod(void *out, int32_t out_dtype, int64_t out_tok_st
  * take SMs as that kernel's blocks finish, schedule their work and start the
  * copies of their first K/V tiles, then wait for that kernel to complete before
  * they read q / k_new / v_new or write anything.  Valid only when the kernel
- * ahead writes none of this launch's pools, block tables or ctx_lens (e.g. it
- * is the previous layer's decode). */
+ * ahead writes none of this launch's pools, block tables, ctx_lens or arrays of
+ * mz_score_mod (e.g. it is the previous layer's decode). */
 #define MZ_LAUNCH_OVERLAP_PREVIOUS 1u
 /* MZ_DECODE_BATCH_INVARIANT: every (sequence, KV head) pair is cut into
  * pieces at fixed pair-relative boundaries (512 tokens), the pieces are
- * handed out by ticket, and a pair's pieces are merged in piece order, so a
- * sequence's output bytes do not depend on its position in the batch or on
- * the other sequences.  The batch-position determinism gate of the
+ * handed out by ticket, and a pair's pieces are merged by sums whose order and
+ * rounding follow from the pair alone, so a sequence's output bytes do not
+ * depend on its position in the batch or on the other sequences.  The batch-position determinism gate of the
  * reference's plan (MLXZ_IMPLEMENTATION_PLAN.md:1058-1059: prefix-cache drift
  * < 1e-4, batch-position determinism bytewise).  Its workspace depends on the
  * table width: size it with mz_paged_decode_workspace_size_ex. */

@@ -420,7 +420,7 @@ struct Sched {
     if constexpr (std::is_same<P, ModParams>::value) {
       // A share costs its warp about 1.3 us a tile, a piece its pair's merging warp
       // 0.1 to 0.4 us: shares below sqrt(n / 5) of n tiles lose more in the merge than
-      // they save (one sequence of 2000 tokens 75 -> 24 us, of 16384 83 -> 61 us); t_s
+      // they save (one sequence of 2000 tokens 75 -> 24 us, of 16384 77 -> 60 us); t_s
       // is tot here, and the last warps get none.
       if (dyn == 0)
         per_s = max(per_s, max(2, static_cast<int>(sqrtf(0.2f * static_cast<float>(longest)))));
@@ -764,7 +764,7 @@ constexpr int kMergeNow = 16;  // rows * pieces up to which a merge runs at once
 // Merge of many pieces: each row's maximum and the pieces' weights first, so that
 // what a piece costs then is a copy and a multiply-add per element, with the next
 // pieces' copies in flight.  Up to MR rows.
-// One sequence of 16384 tokens (73 pieces a pair) 61 -> 40 us, of 2000 24 -> 19;
+// One sequence of 16384 tokens (73 pieces a pair) 60 -> 40 us, of 2000 24 -> 19;
 // few pieces, which one round trip of the staged merge takes, are left to it.
 constexpr int kWeighted = 6;  // pieces from which on it runs
 

@@ -1,6 +1,6 @@
 // Entry points by number, their arguments in 8-byte slots: a caller whose foreign
-// function interface pays per argument (40 of them: 8 us from Python) packs them
-// in one step (1 us) and passes two.
+// function interface pays per argument (40 of them: 3.8 us from Python) packs
+// them in one step and passes two (1.1 us).
 #include <cstring>
 #include <limits>
 #include <tuple>

@@ -330,7 +330,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
         }
       }
     }
-    uint32_t ph[RG][2], pl[RG][2];  // P^T as B fragments, and bf16's low part
+    // P^T as B fragments: fp16 has 11 bits of P in one part, as in the unmodified
+    // kernel (2^-11 of an output, an fp16 output's own rounding, seen in fp32 ones);
+    // bf16's 8 are too few for its outputs, so its low part makes them 16
+    uint32_t ph[RG][2], pl[RG][2];
 #pragma unroll
     for (int x = 0; x < RG; ++x) {
       float(&sc)[4] = sacc[x][0];

@@ -29,7 +29,7 @@
 // that polls both streams' barriers (425 us with S first, 482 us with P.V first);
 // the MMAs issued by one lane's branch instead of an elected lane (414 us);
 // exponentials against the running maximum as it is while the tile's is found,
-// redone where it moves (365 us).  P in one bf16 part would give 321 us.
+// redone where it moves (365 us).  P in one bf16 part would give 310 us.
 //
 // TMEM columns of stream s: O at 128 s, S buffers at 256 + 128 s, 64 each.  P
 // takes its scores' place: hi parts in the first 32 columns, lo in the last.
@@ -44,8 +44,10 @@
 // O there and writes the joined columns that are its share.  No workspace, no
 // second launch.  With a cap of 50, 32 tokens at 16384 take 44 us (338 us as whole
 // items), 64 at 2000 22 us (51), 32 at 600 19 us (22); 64 behind a window of 4096
-// 25 us (73).  Joining costs 3 to 5 us, so a part has two tiles at least: parts of
-// four made 32 tokens at 600 22 us and 1 at 400 17 instead of 14 us.  Not kept: the
+// 25 us (73).  Joining costs 3 to 5 us, so clusters
+// are no larger than gives two tiles a part of the longest item that the table or
+// the window allows (parts of four made 32 tokens at 600 22 us and 1 at 400 17
+// instead of 14 us); a shorter item's parts may have one tile, or none.  Not kept: the
 // odd last item of a CTA among many shared by its two streams in the same way
 // (window 350 against 360 us, but documents 112 against 105, a cap on 256 items of
 // 8192 keys 252 against 232: a stream alone runs faster than one of two).
@@ -713,7 +715,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float a = fast_exp2(xa), z = fast_exp2(xe);
             const uint64_t az = f2_pack(a, z);
             l2[w & 3] = f2_add(l2[w & 3], az);
-            hi[w] = pack2<BF16>(a, z);
+            hi[w] = pack2<BF16>(a, z);  // fp16 has 11 bits of P in one part, bf16 16 in two
             if constexpr (BF16) {
               // the rest of P, so that P.V carries 16 bits of it
               float ra, rz;

@@ -50,7 +50,9 @@ __device__ __forceinline__ float tanh_mod(float z) {
 }
 
 // cap_log2 * tanh(z_scale * s): 1 - 2 / (e^(2 z) + 1) is off by 2.4e-7 at most, so
-// by less than 2^-12 in the scores up to a cap of 1000; above it by tanh_mod.
+// by less than 2^-12 in the scores up to a cap of 1000.  Decode takes it for every
+// score up to that cap (prefill only for tiles with scores beyond half the cap,
+// the cubic below for the rest), tanh_mod above it.
 __device__ __forceinline__ float rcp_approx(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -171,13 +171,14 @@ class PagedDecodeStep:
     already on the device; ``step_host`` is the end-to-end form that copies
     them from (pinned) host memory and copies the output back.
     ``batch_invariant``: every sequence's output bytes are independent of the
-    batch (each (sequence, KV head) pair is computed whole by one warp).
+    batch (each (sequence, KV head) pair is cut every 512 of the tokens it sees
+    and its pieces are merged by the same sums whatever else runs).
 
     ``rope``: one QKNormRope or one per layer, applied to q and the new keys as
     projected, at ``rope_positions`` (int32 ``[B]`` or ``[axes, B]``, which the
     caller keeps up to date; default: the write positions).  ``softcap``,
     ``alibi_slopes``, ``window``, ``sink_tokens``, ``prefix_lens`` and
-    ``first_keys`` as in ``ops.paged_decode``.
+    ``first_keys`` as in ``ops.paged_decode``, the same for every layer.
     """
 
     def __init__(self, store: PagedKVStore, seq_ids: list[str], n_heads: int,
@@ -261,7 +262,8 @@ class PagedDecodeStep:
         """Append this step's token of layer l and attend, one launch (device
         tensors).  Layers after the first may start while the previous layer's
         launch finishes (it writes none of this layer's pools, and the tables
-        and lengths change only between steps)."""
+        and lengths change only between steps); with ``rope`` its launch stands
+        between them, and the attention starts under its end alone."""
         st = self.store
         q, k_new = self._turn(l, q, k_new)
         ops.paged_append_decode(q, st.k_pool(l), st.v_pool(l), k_new, v_new, self.tables,

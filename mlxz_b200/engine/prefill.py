@@ -94,7 +94,8 @@ class PagedPrefillStep:
     ``rope_positions`` (int32 ``[T]`` or ``[axes, T]``; default: each token's
     position in its sequence).  ``softcap``, ``alibi_slopes``, ``window``,
     ``sink_tokens`` and ``first_keys`` (int32 ``[T]``) as in
-    ``ops.paged_prefill``; ``prefix_lens``: one number per chunk."""
+    ``ops.paged_prefill``; ``prefix_lens``: one number per chunk.  They are the
+    same for every layer."""
 
     def __init__(self, store: PagedKVStore, chunks: list[tuple[str, int]], n_heads: int,
                  scale: float | None = None,

@@ -528,8 +528,10 @@ def paged_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
     softcap)``; ``alibi_slopes`` float32 ``[Hq]`` subtracts ``slope * distance``;
     a token sees the last ``window`` keys (0: all), not those before
     ``first_keys[b]`` (its document's start), and in any case the first
-    ``sink_tokens`` and the first ``prefix_lens[b]``.  A token that sees no key
-    gets zeros; blocks that no token sees need no valid table entry.
+    ``sink_tokens`` (the sequence's, not its documents') and the first
+    ``prefix_lens[b]``.  A token that sees no key gets zeros; blocks behind those
+    first ones and below the lowest key that window and ``first_keys`` leave to
+    the sequence's tokens need no valid table entry.
     """
     n_blocks, Hkv, bs, D = _check_pools(k_pool, v_pool)
     if q.dtype != k_pool.dtype:
@@ -610,7 +612,8 @@ def paged_append_decode(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Ten
     over the first ``ctx_lens[b]`` tokens (one launch).  ``overlap_previous``:
     the launch may start while the kernel ahead of it on the stream runs
     (MZ_LAUNCH_OVERLAP_PREVIOUS) -- only when that kernel writes none of the
-    pools, ``block_tables`` or ``ctx_lens``.  ``batch_invariant``: each
+    pools, ``block_tables``, ``ctx_lens``, ``alibi_slopes``, ``prefix_lens`` or
+    ``first_keys``.  ``batch_invariant``: each
     sequence's output bytes are independent of the rest of the batch
     (MZ_DECODE_BATCH_INVARIANT).  Modified scores and masks as in
     ``paged_decode``."""
