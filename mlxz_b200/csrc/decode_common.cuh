@@ -1013,6 +1013,14 @@ struct WsLayout {
   int max_chunks;
 };
 
+// Tables whose tokens a kernel's int arithmetic can count: positions run up to
+// `ahead` past the table's last one (block ids loaded ahead, a tile's end).
+inline int check_capacity(int32_t max_blocks, int32_t bs, int ahead, const char *fn) {
+  if ((int64_t)max_blocks * bs > (int64_t(1) << 31) - ahead)
+    return fail(MZ_ERR_UNSUPPORTED, "%s: tables span 2^31 or more tokens", fn);
+  return MZ_OK;
+}
+
 inline size_t align256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 
 // Workspace for W warps: per-pair counters + 2 scheduler words, then (m, l)

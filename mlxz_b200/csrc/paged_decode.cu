@@ -507,6 +507,7 @@ int validate(const DecodeArgs &a, const char *fn, int64_t *warps, WsLayout *ws) 
   const int64_t rows_total = a.n_blocks * a.Hkv * a.bs;
   if (rows_total >= (int64_t(1) << 31))
     return fail(MZ_ERR_UNSUPPORTED, "%s: pool has >= 2^31 rows", fn);
+  if (int rc = check_capacity(a.max_blocks, a.bs, 1024, fn)) return rc;
   if ((int64_t)a.B * a.Hkv * a.max_blocks * (a.bs / kTileTok) >= (int64_t(1) << 30))
     return fail(MZ_ERR_UNSUPPORTED, "%s: more than 2^30 tiles of context", fn);
   const int device = current_device();

@@ -1056,6 +1056,8 @@ extern "C" int mz_paged_prefill(void *out, int32_t out_dtype, int64_t out_tok_st
   CUtensorMap tk, tv;
   PParams p;
   bool empty = false;
+  // (block ids are loaded up to 1135 tokens behind the last one)
+  if (int rc = decode::check_capacity(max_blocks_per_seq, block_size, 2048, fn)) return rc;
   if (int rc = prepare(&p, &tk, &tv, &empty, 7, out, out_dtype, out_tok_stride, out_head_stride, q,
                        q_tok_stride, q_head_stride, n_rows, q_start, q_len, max_q_len, k_pool,
                        v_pool, block_tables, max_blocks_per_seq, ctx_lens, n_seqs, n_heads,

@@ -1006,6 +1006,7 @@ extern "C" int mz_paged_decode_q(void *out, int32_t out_dtype, int64_t out_seq_s
   const int ob = out_dtype == MZ_DTYPE_F32 ? 8 : 4;
   if (!aligned(out, ob) || (out_seq_stride & 1) || (out_tok_stride & 1) || (out_head_stride & 1))
     return fail(MZ_ERR_ALIGNMENT, "%s: out needs %d-byte alignment and even strides", fn, ob);
+  if (int rc = check_capacity(max_blocks_per_seq, block_size, 1024, fn)) return rc;
   if ((int64_t)n_seqs * n_kv_heads * max_blocks_per_seq * (block_size / kTileTok) >= (int64_t(1) << 30))
     return fail(MZ_ERR_UNSUPPORTED, "%s: more than 2^30 tiles of context", fn);
   const int device = current_device();

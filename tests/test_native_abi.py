@@ -62,3 +62,22 @@ def test_missing_library_fails_loudly(monkeypatch, tmp_path):
     monkeypatch.setattr(_native, "_lib", None)
     with pytest.raises(_native.NativeLibraryError):
         _native.lib()
+
+
+@pytest.mark.parametrize("width,bs", [(1 << 27, 16), (1 << 21, 1024), ((1 << 28) + 64, 16)])
+def test_tables_of_2_to_31_tokens_are_refused(lib, width, bs):
+    """Positions are ints in the kernels: a table of 2^31 tokens has a capacity
+    that is negative or small there."""
+    p = ctypes.c_void_p(256)  # never read: every call below is refused first
+    q = (p, 1, 512, 64, p, 512, 64, 4, p, p, 4, p, p, p, width, p, 1, 8, 2, 64, bs, 4, 0.125, 1,
+         None, None)
+    assert lib.mz_paged_prefill(*q) == _native.MZ_ERR_UNSUPPORTED
+    assert "2^31" in _native.last_error()[1]
+    assert lib.mz_paged_decode(p, 1, 512, 512, 64, p, 512, 512, 64, 1, p, p, p, width, p, 1, 8, 2,
+                               64, bs, 4, 0.125, 1, 4, p, 1 << 30, None,
+                               None) == _native.MZ_ERR_UNSUPPORTED
+    assert "2^31" in _native.last_error()[1]
+    assert lib.mz_paged_decode_q(p, 1, 512, 512, 64, p, 512, 512, 64, 1, p, p, p, p, p, p, p,
+                                 width, p, 1, 8, 2, 64, bs, 4, 8, 64, 0.125, 1, 4, p, 1 << 30, None,
+                                 None) == _native.MZ_ERR_UNSUPPORTED
+    assert "2^31" in _native.last_error()[1]
